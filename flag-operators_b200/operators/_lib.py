@@ -7,6 +7,7 @@ raises instead of computing the result some other way.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -83,12 +84,27 @@ _SIGS = {
     "fo_gdr_bwd_workspace_bytes": [_i64, _i64, _i64, _i64, _i64p],
     "fo_gdr_bwd": [_c_void_p] * 14 + [_i64, _i64, _i64, _i64, _int, _int, _c_void_p,
                                       _i64, _c_void_p],
+    "fo_glr_fwd": [_c_void_p] * 9 + [_i64, _i64, _i64, _i64p, _f32, _int, _int, _c_void_p],
+    "fo_glr_step": [_c_void_p] * 6 + [_i64, _i64, _i64p, _f32, _int, _int, _c_void_p],
+    "fo_glr_bwd_workspace_bytes": [_i64, _i64, _i64, _i64p],
+    "fo_glr_bwd": [_c_void_p] * 13 + [_i64, _i64, _i64, _i64p, _f32, _int, _int, _c_void_p, _i64,
+                                      _c_void_p],
+    "fo_residual_rms_norm_fwd": [_c_void_p] * 6 + [_f32] + [_c_void_p] * 4 + [_i64] * 5 + [
+        _f32, _int, _int, _int, _c_void_p],
+    "fo_residual_rms_norm_bwd_workspace_bytes": [_i64, _i64, _i64p],
+    "fo_residual_rms_norm_bwd": [_c_void_p] * 8 + [_f32] + [_c_void_p] * 8 + [_i64] * 5 + [
+        _int, _int, _int, _c_void_p, _i64, _c_void_p],
+    "fo_embedding_fwd": [_c_void_p] * 3 + [_i64] * 4 + [_f32, _int, _int, _c_void_p],
+    "fo_embedding_bwd_workspace_bytes": [_i64, _i64, _i64, _i64p],
+    "fo_embedding_bwd": [_c_void_p] * 3 + [_i64] * 4 + [_f32, _int, _int, _c_void_p, _i64,
+                                                        _c_void_p],
     "fo_median_timeouts": [_c_void_p],
     "fo_tc05_selftest": [_c_void_p, _c_void_p, _c_void_p, _i64, _i64, _int, _int, _c_void_p],
 }
 
 _lock = threading.Lock()
 _lib = None
+_SAME_DEVICE = contextlib.nullcontext()
 
 
 class LibraryNotLoaded(RuntimeError):
@@ -153,6 +169,13 @@ def ptr(t: torch.Tensor | None):
 
 def stream_of(t: torch.Tensor):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+def on_device(t: torch.Tensor):
+    """Makes t's device the current one for a launch (a launch goes to the current device)."""
+    if t.get_device() == torch.cuda.current_device():
+        return _SAME_DEVICE
+    return torch.cuda.device(t.device)
 
 
 def i64_array(vals) -> ctypes.Array:

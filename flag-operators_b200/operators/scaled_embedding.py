@@ -1,0 +1,140 @@
+"""scaled_embedding — embedding lookup with a scale, and its gradient.
+
+    scaled_embedding(ids, weight, scale=1.0, *, padding_idx=None) -> out [*ids.shape, N]
+    scaled_embedding_backward(dout, ids, num_embeddings, scale=1.0, *, padding_idx=None) -> dweight
+
+    out[t] = scale * weight[ids[t]] ,  dweight[v] = scale * sum of dout[t] over ids[t] == v
+
+ids: int64 or int32 of any shape; weight: [V, N] fp32 / fp16 / bf16.  The product is taken in
+fp32 and rounded once; the gradient's sums are in fp32 and in a fixed order (tokens sorted by id,
+no floating-point atomics), so it is the same in every run.  The gradient is dense: all of its
+V rows are written.  Rows of `padding_idx` (negative counts from the end) are looked up as any
+other and get no gradient.
+
+As scatter_reduce does with its index, ids outside [0, V) are not read: they give a row of
+zeros and no gradient, and with FLAGOPS_CHECK_INDEX=1 the wrapper synchronises and raises
+IndexError.  scaled_embedding is differentiable, once, in weight.
+"""
+from __future__ import annotations
+
+import ctypes
+import logging
+import os
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+logger = logging.getLogger(__name__)
+
+
+def _check_ids(op, ids, V):
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"{op}: ids must be int64 or int32, got {ids.dtype}")
+    if os.environ.get("FLAGOPS_CHECK_INDEX") == "1" and ids.numel() \
+            and bool(((ids < 0) | (ids >= V)).any()):
+        raise IndexError(f"{op}: id out of range [0, {V})")
+
+
+def _check_dtype(op, t):
+    if t.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise TypeError(f"{op}: dtype {t.dtype} is not supported")
+
+
+def _padding(op, padding_idx, V):
+    if padding_idx is None:
+        return -1
+    p = int(padding_idx)
+    if not -V <= p < V:
+        raise ValueError(f"{op}: padding_idx {p} out of range for {V} rows")
+    return p + V if p < 0 else p
+
+
+def _forward(ids, weight, scale):
+    V, N = weight.shape
+    out = torch.empty((*ids.shape, N), dtype=weight.dtype, device=weight.device)
+    with _lib.on_device(weight):
+        _lib.call("fo_embedding_fwd", _lib.ptr(ids), _lib.ptr(weight), _lib.ptr(out), ids.numel(),
+                  V, N, weight.stride(0) if V > 1 else N, scale, _lib.dtype_code(weight.dtype),
+                  _lib.dtype_code(ids.dtype), _lib.stream_of(weight))
+    return out
+
+
+def _backward(dout, ids, V, scale, padding_idx):
+    N, T = dout.shape[-1], ids.numel()
+    dout = dout.contiguous()
+    dw = torch.empty((V, N), dtype=dout.dtype, device=dout.device)
+    nbytes = ctypes.c_int64(0)
+    with _lib.on_device(dout):
+        _lib.call("fo_embedding_bwd_workspace_bytes", T, V, N, ctypes.byref(nbytes))
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dout.device) \
+            if nbytes.value else None
+        _lib.call("fo_embedding_bwd", _lib.ptr(dout), _lib.ptr(ids), _lib.ptr(dw), T, V, N,
+                  padding_idx, scale, _lib.dtype_code(dout.dtype), _lib.dtype_code(ids.dtype),
+                  _lib.ptr(ws), nbytes.value, _lib.stream_of(dout))
+    return dw
+
+
+class _ScaledEmbedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, weight, scale, padding_idx):
+        ctx.save_for_backward(ids)
+        ctx.args = (weight.shape[0], scale, padding_idx)
+        ctx.dtype = weight.dtype
+        return _forward(ids, weight, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        (ids,) = ctx.saved_tensors
+        return None, _backward(dout.to(ctx.dtype), ids, *ctx.args), None, None
+
+
+def scaled_embedding(
+    ids: torch.Tensor,
+    weight: torch.Tensor,
+    scale: float = 1.0,
+    *,
+    padding_idx: int | None = None,
+) -> torch.Tensor:
+    """scale * weight[ids]; see the module's documentation."""
+    logger.debug("FLAG-OPS SCALED_EMBEDDING")
+    op = "scaled_embedding"
+    _lib.require_cuda(weight, op)
+    if weight.dim() != 2:
+        raise ValueError(f"{op}: weight must be [V, N], got shape {tuple(weight.shape)}")
+    _check_dtype(op, weight)
+    if ids.device != weight.device:
+        raise ValueError(f"{op}: ids must be on the same device as weight")
+    V = weight.shape[0]
+    _check_ids(op, ids, V)
+    padding_idx = _padding(op, padding_idx, V)
+    ids = ids.contiguous()
+    if weight.stride(1) != 1 and weight.shape[1] > 1:
+        weight = weight.contiguous()
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return _ScaledEmbedding.apply(ids, weight, float(scale), padding_idx)
+    return _forward(ids, weight, float(scale))
+
+
+def scaled_embedding_backward(
+    dout: torch.Tensor,
+    ids: torch.Tensor,
+    num_embeddings: int,
+    scale: float = 1.0,
+    *,
+    padding_idx: int | None = None,
+) -> torch.Tensor:
+    """d weight [num_embeddings, N] of scaled_embedding, in dout's dtype."""
+    op = "scaled_embedding_backward"
+    _lib.require_cuda(dout, op)
+    _check_dtype(op, dout)
+    V = int(num_embeddings)
+    if V < 0 or dout.dim() < 1 or dout.shape[:-1] != ids.shape:
+        raise ValueError(f"{op}: dout shape {tuple(dout.shape)} does not fit ids {tuple(ids.shape)} and "
+                         f"{V} rows")
+    if ids.device != dout.device:
+        raise ValueError(f"{op}: ids must be on the same device as dout")
+    _check_ids(op, ids, V)
+    return _backward(dout, ids.contiguous(), V, float(scale), _padding(op, padding_idx, V))

@@ -1,5 +1,5 @@
 /*
- * flagops.h — C ABI of the B200 (sm_100a) five-operator kernel set.
+ * flagops.h — C ABI of the B200 (sm_100a) kernel set.
  *
  * Every entry point takes raw device pointers, int64 sizes, dtype codes and a
  * cudaStream_t passed as void*.  Nothing here allocates device memory (only
@@ -61,6 +61,13 @@ enum fo_reduction {
   FO_RED_NONE = 0,
   FO_RED_MEAN = 1,
   FO_RED_SUM = 2
+};
+
+/* gate activations of fo_residual_rms_norm_* */
+enum fo_gate_act {
+  FO_ACT_NONE = 0,
+  FO_ACT_SILU = 1,
+  FO_ACT_SIGMOID = 2
 };
 
 /* Message of the last failed call on this thread ("" if none). */
@@ -382,6 +389,92 @@ FO_API int fo_gdr_bwd(const void* q, const void* k, const void* v, const void* b
                       void* dq, void* dk, void* dv, void* dbeta, void* dg, float* dh0,
                       int64_t B, int64_t H, int64_t L, int64_t D, int dtype, int gate_dtype,
                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* gated linear recurrence (no reference counterpart)                        */
+/* ------------------------------------------------------------------------ */
+/*
+ * h_t = a_t h_{t-1} + b_t for every channel of x, g, beta [B, L, C].
+ * decay == NULL: a_t = g_t, b_t = beta_t x_t.  decay [C] fp32: g and beta are logits,
+ * a_t = exp(-scale softplus(decay) sigmoid(g_t)), b_t = sqrt(1 - a_t^2) sigmoid(beta_t) x_t.
+ * reset [B, L] bytes or NULL: a_t = 0 where not zero.  h0 / hT: [B, C] fp32 states or NULL.
+ * h: [B, L, C] contiguous, dtype.  gate_dtype is dtype or FO_F32.
+ * strides: batch and step strides of x, g, beta in elements (six numbers); channels are
+ * contiguous.  ckpt, for the backward: [B, ceil(L / FO_GLR_CHECKPOINT), C] fp32 or NULL, the
+ * state in front of every FO_GLR_CHECKPOINT-th step.  B <= 65535.
+ */
+#define FO_GLR_CHECKPOINT 64
+FO_API int fo_glr_fwd(const void* x, const void* g, const void* beta, const float* decay,
+                      const float* h0, const uint8_t* reset, void* h, float* hT, float* ckpt,
+                      int64_t B, int64_t L, int64_t C, const int64_t* strides, float scale,
+                      int dtype, int gate_dtype, void* stream);
+/* One step of B sequences: x, g, beta [B, C] (row strides: three numbers), state [B, C] fp32
+ * overwritten with h_t, h [B, C] = h_t in dtype. */
+FO_API int fo_glr_step(const void* x, const void* g, const void* beta, const float* decay,
+                       float* state, void* h, int64_t B, int64_t C, const int64_t* strides,
+                       float scale, int dtype, int gate_dtype, void* stream);
+/*
+ * Gradients given dh = dL/dh [B, L, C] and dhT = dL/dh_T ([B, C] fp32 or NULL): dx, dg, dbeta
+ * [B, L, C] contiguous, dh0 [B, C] fp32 or NULL, ddecay [C] fp32 or NULL (needs the workspace:
+ * fo_glr_bwd_workspace_bytes).  Fixed-order sums.
+ */
+FO_API int fo_glr_bwd_workspace_bytes(int64_t B, int64_t L, int64_t C, int64_t* bytes);
+FO_API int fo_glr_bwd(const void* x, const void* g, const void* beta, const float* decay,
+                      const uint8_t* reset, const float* ckpt, const void* dh, const float* dhT,
+                      void* dx, void* dg, void* dbeta, float* dh0, float* ddecay, int64_t B,
+                      int64_t L, int64_t C, const int64_t* strides, float scale, int dtype,
+                      int gate_dtype, void* workspace, int64_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* residual RMS norm (no reference counterpart)                              */
+/* ------------------------------------------------------------------------ */
+/*
+ * u = act(gate) * y * inv1 * post_weight,  res_out = residual + s * u,
+ * out = res_out * inv2 * weight (res_out before it is rounded), inv = 1/sqrt(mean(row^2) + eps).
+ * y, residual, gate: [M, N] with row strides y_ld, r_ld, g_ld; out, res_out: contiguous, all of
+ * dtype.  post_weight NULL: no first norm; gate NULL (and act FO_ACT_NONE): no gate;
+ * scale_vec [N] or NULL (then the number scale).  Vectors are of w_dtype: dtype or FO_F32.
+ * inv1, inv2: [M] fp32 for the backward, or NULL.  out and res_out must not overlap the inputs.
+ */
+FO_API int fo_residual_rms_norm_fwd(const void* y, const void* residual, const void* weight,
+                                    const void* post_weight, const void* gate,
+                                    const void* scale_vec, float scale, void* out, void* res_out,
+                                    float* inv1, float* inv2, int64_t M, int64_t N, int64_t y_ld,
+                                    int64_t r_ld, int64_t g_ld, float eps, int act, int dtype,
+                                    int w_dtype, void* stream);
+/*
+ * Gradients given dout, dres ([M, N] contiguous; NULL is zero): dy, dr, dgate [M, N] contiguous,
+ * dw, dwp, ds [N] of w_dtype (dgate, dwp, ds are NULL where their input is).  Fixed-order sums.
+ */
+FO_API int fo_residual_rms_norm_bwd_workspace_bytes(int64_t M, int64_t N, int64_t* bytes);
+FO_API int fo_residual_rms_norm_bwd(const void* dout, const void* dres, const void* y,
+                                    const void* residual, const void* weight,
+                                    const void* post_weight, const void* gate,
+                                    const void* scale_vec, float scale, const float* inv1,
+                                    const float* inv2, void* dy, void* dr, void* dgate, void* dw,
+                                    void* dwp, void* ds, int64_t M, int64_t N, int64_t y_ld,
+                                    int64_t r_ld, int64_t g_ld, int act, int dtype, int w_dtype,
+                                    void* workspace, int64_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* scaled embedding (no reference counterpart)                               */
+/* ------------------------------------------------------------------------ */
+/*
+ * out[t, :] = scale * weight[ids[t], :] (rounded once); zeros where ids[t] is outside [0, V).
+ * ids: [T] int64 or int32; weight: [V, N] with row stride ld; out: [T, N] contiguous.
+ */
+FO_API int fo_embedding_fwd(const void* ids, const void* weight, void* out, int64_t T, int64_t V,
+                            int64_t N, int64_t ld, float scale, int dtype, int index_dtype,
+                            void* stream);
+/*
+ * dw[v, :] = scale * sum of dout[t, :] over the t with ids[t] == v, in fp32 and in a fixed order;
+ * every row of dw [V, N] is written.  Ids outside [0, V) and equal to padding_idx add nothing
+ * (padding_idx -1: none).
+ */
+FO_API int fo_embedding_bwd_workspace_bytes(int64_t T, int64_t V, int64_t N, int64_t* bytes);
+FO_API int fo_embedding_bwd(const void* dout, const void* ids, void* dw, int64_t T, int64_t V,
+                            int64_t N, int64_t padding_idx, float scale, int dtype,
+                            int index_dtype, void* workspace, int64_t ws_bytes, void* stream);
 
 /* Number of hand-off waits of the producer/consumer median kernel (rows of
  * 1024 < N <= 2048) that ran out of polls since the library was loaded (0 in a
