@@ -8,163 +8,557 @@
 //
 // Backward, with D_t = dL/dh_t in total: D_t = dh_t + a_{t+1} D_{t+1} (D_{L-1} += dL/dh_T),
 //   values:  dg = D h_{t-1},  dbeta = D x,  dx = D beta
-//   logits:  du = D (a h_{t-1} - a^2 / m * i x),  dg = du u (1 - sigmoid(g)),
-//            ddecay = -scale sigmoid(decay) sum du sigmoid(g),
-//            dx = D m i,  dbeta = D m x i (1 - i)
+//   logits:  du = D (a h_{t-1} - a^2 / (1 - a^2) b),  dg = du u (1 - sigmoid(g)),
+//            ddecay = sigmoid(decay) / softplus(decay) * sum du u,
+//            dx = D m i,  dbeta = D b (1 - i)
 //   and dg = du = 0 at a reset step; dh0 = a_0 D_0.
 // The states h_{t-1} are recomputed in fp32 from the state the forward keeps in front of every
 // FO_GLR_CHECKPOINT-th step: recomputing costs no traffic beyond x, g and beta, which the
 // backward reads anyway, and gradients do not see the output's rounding to 16 bits.
-//
 // All of it is held in fp32; h and the gradients are rounded once when they are written.
+//
+// Split.  Time is cut into tiles of 64 steps, channels into slabs of 32 lanes (two channels a lane
+// where C, the strides and the addresses allow it, so a warp's row is one 128-byte line in 16
+// bits).  A CTA's 8 warps take 8 consecutive steps of a tile each, held in registers: over its
+// steps a warp is the map s -> A s + H (backward: R -> A R + Q), the 8 maps meet in shared memory,
+// and each warp then walks its steps once from the state that enters them.  So the axis is
+// walked 64 steps at a time and every input is read once.  Where B * C gives too few CTAs to fill
+// the GPU, up to 8 CTAs of a cluster take consecutive tiles and exchange their maps through
+// distributed shared memory, one cluster barrier a round.  The next tiles' inputs are on their way
+// meanwhile: a ring of kStages tiles in shared memory, each thread copying (cp.async) just the
+// elements that it will read, so that the ring needs no barrier.
+#include <type_traits>
+
 #include "gates.cuh"
 
 namespace fo {
 namespace {
 
-constexpr int kCkpt = FO_GLR_CHECKPOINT;
+constexpr int kSteps = 8;                  // steps of a thread in a tile
+constexpr int kWarps = 8;                  // warps of a CTA, along time
+constexpr int kTile = kSteps * kWarps;     // steps of a CTA in a round
+constexpr int kStages = 2;                 // tiles of the ring
+constexpr int kThreads = 32 * kWarps;
+static_assert(kTile == FO_GLR_CHECKPOINT, "a tile begins at a checkpoint");
 
 struct Strides {
   int64_t xb, xl, gb, gl, bb, bl;  // batch and step strides of x, g, beta, in elements
 };
 
-// 1 - e^{-w} for w >= 0.  Below 0.5 by its series to w^8 (next term / first term < 4e-9 there),
-// since 1 - e^{-w} loses 1/w in relative precision; above, the subtraction loses at most 2.5x.
-__device__ __forceinline__ float one_minus_exp(float w, float e) {
-  float p = fmaf(w, -1.f / 40320.f, 1.f / 5040.f);
-  p = fmaf(w, -p, 1.f / 720.f);
-  p = fmaf(w, -p, 1.f / 120.f);
-  p = fmaf(w, -p, 1.f / 24.f);
-  p = fmaf(w, -p, 1.f / 6.f);
-  p = fmaf(w, -p, 0.5f);
-  p = fmaf(w, -p, 1.f);
-  return w < 0.5f ? w * p : 1.f - e;
+// (1 - e^{-w}) / w on [0, 1/2]: interpolation at the six Chebyshev nodes, relative error 3e-9.
+// Above 1/2 the subtraction 1 - e^{-w} loses at most a factor 2.5; below, it would lose 1 / w.
+template <typename F>
+__device__ __forceinline__ F one_minus_exp(F w, F e) {
+  F p = fma_(w, all_<F>(-1.1234042e-3f), all_<F>(8.1896139e-3f));
+  p = fma_(w, p, all_<F>(-4.1630074e-2f));
+  p = fma_(w, p, all_<F>(0.16666242f));
+  p = fma_(w, p, all_<F>(-0.49999982f));
+  p = fma_(w, p, all_<F>(1.f));
+  return map_([](float w_, float s, float l) { return w_ < 0.5f ? s : l; }, w, mul_(w, p),
+              fma_(e, all_<F>(-1.f), all_<F>(1.f)));
+}
+__device__ __forceinline__ float sqrt_(float x) {
+  float y;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-// Per-channel -scale * softplus(decay) (the log decay of a fully open gate).
-__device__ __forceinline__ float log_decay(float decay, float scale) {
-  return -scale * (decay > 20.f ? decay : log1pf(expf(decay)));
+// softplus(decay), the rate of a fully open gate
+__device__ __forceinline__ float softplus(float decay) {
+  return decay > 20.f ? decay : log1pf(expf(decay));
 }
 
-struct Gate {
-  float a, b;        // h_t = a h_{t-1} + b
-  float u, s, c;     // log a, sigmoid(g), 1 - sigmoid(g)
-  float m, i, ci;    // sqrt(1 - a^2), sigmoid(beta), 1 - sigmoid(beta)
+// The state s behind a segment that maps it to A s + H.  A zero on either side leaves H, so that an
+// A that left the fp32 range over an empty state, or a state before a reset, adds nothing.
+__device__ __forceinline__ float through1(float s, float A, float H) {
+  return s == 0.f || A == 0.f ? H : fmaf(A, s, H);
+}
+template <typename F> __device__ __forceinline__ F through(F s, F A, F H) {
+  return map_(through1, s, A, H);
+}
+
+// ---------------------------------------------------------------------------
+// Elements of a lane: V channels of T in memory, F (float or float2) in registers
+// ---------------------------------------------------------------------------
+template <int V> struct Lane;
+template <> struct Lane<1> { using F = float; };
+template <> struct Lane<2> { using F = float2; };
+
+template <int BYTES> struct Word;
+template <> struct Word<2> { using type = uint16_t; };
+template <> struct Word<4> { using type = uint32_t; };
+template <> struct Word<8> { using type = uint2; };
+
+template <typename T, int V> struct Elem {
+  static constexpr int kBytes = V * (int)sizeof(T);
+  using W = typename Word<kBytes>::type;
+  using F = typename Lane<V>::F;
+  static __device__ __forceinline__ F load(const void* p) {
+    const W w = *reinterpret_cast<const W*>(p);
+    const T* e = reinterpret_cast<const T*>(&w);
+    if constexpr (V == 1) return to_f<T>(e[0]);
+    else return make_float2(to_f<T>(e[0]), to_f<T>(e[1]));
+  }
+  static __device__ __forceinline__ void store(T* p, F v) {
+    W w;
+    T* e = reinterpret_cast<T*>(&w);
+    if constexpr (V == 1) {
+      e[0] = from_f<T>(v);
+    } else {
+      e[0] = from_f<T>(v.x);
+      e[1] = from_f<T>(v.y);
+    }
+    *reinterpret_cast<W*>(p) = w;
+  }
+  // global -> shared without waiting (2-byte elements have no such copy: through a register)
+  static __device__ __forceinline__ void copy(void* smem, const T* p) {
+    if constexpr (kBytes == 2) {
+      *reinterpret_cast<W*>(smem) = *reinterpret_cast<const W*>(p);
+    } else {
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(
+                       (uint32_t)__cvta_generic_to_shared(smem)),
+                   "l"(p), "n"(kBytes)
+                   : "memory");
+    }
+  }
+};
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// ---------------------------------------------------------------------------
+// Clusters
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+__device__ __forceinline__ void store_remote(void* smem, uint32_t cta, float v) {
+  asm volatile(
+      "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, %1;\n\t"
+      "st.shared::cluster.f32 [r], %2;\n\t}" ::"r"((uint32_t)__cvta_generic_to_shared(smem)),
+      "r"(cta), "f"(v)
+      : "memory");
+}
+__device__ __forceinline__ void store_remote(void* smem, uint32_t cta, float2 v) {
+  asm volatile(
+      "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, %1;\n\t"
+      "st.shared::cluster.v2.f32 [r], {%2, %3};\n\t}" ::"r"((uint32_t)__cvta_generic_to_shared(smem)),
+      "r"(cta), "f"(v.x), "f"(v.y)
+      : "memory");
+}
+
+// The maps of a round: of the CTA's warps, and (clusters) of the cluster's CTAs.  Two copies,
+// used in turn: a copy is written again only after a barrier that every reader of it has passed.
+template <typename F, bool CLUSTER> struct Maps {
+  F A[2][kWarps][32], H[2][kWarps][32];
+  F cA[2][CLUSTER ? 8 : 1][32], cH[2][CLUSTER ? 8 : 1][32];
 };
 
-template <bool LOGITS>
-__device__ __forceinline__ Gate gate_of(float x, float g, float beta, float rate, bool reset) {
-  Gate q;
-  if (!LOGITS) {
-    q.a = reset ? 0.f : g;
-    q.b = beta * x;
-    return q;
+// From this warp's map (A, H) and the state S in front of the round: the state in front of
+// this warp's steps; S becomes the state behind the round.  REVERSE walks the warps and CTAs from
+// the last to the first.  entering: the state in front of the CTA's tile.
+template <typename F, bool CLUSTER, bool REVERSE>
+__device__ __forceinline__ F carry_in(Maps<F, CLUSTER>& m, int parity, F A, F H, F& S, F& entering) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  m.A[parity][w][lane] = A;
+  m.H[parity][w][lane] = H;
+  __syncthreads();
+  if constexpr (CLUSTER) {
+    const uint32_t n = cluster_size(), me = cluster_rank();
+    if (w < (int)n) {  // warp w hands the CTA's map to CTA w
+      F a = all_<F>(1.f), h = all_<F>(0.f);
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        const int q = REVERSE ? kWarps - 1 - k : k;
+        const F ak = m.A[parity][q][lane];
+        h = through(h, ak, m.H[parity][q][lane]);
+        // 0 once any factor is 0, whatever the others are
+        a = map_([](float x, float y) { return x == 0.f || y == 0.f ? 0.f : x * y; }, a, ak);
+      }
+      store_remote(&m.cA[parity][me][lane], w, a);
+      store_remote(&m.cH[parity][me][lane], w, h);
+    }
+    cluster_barrier();
+    F mine = S;
+    for (uint32_t k = 0; k < n; ++k) {
+      const uint32_t q = REVERSE ? n - 1 - k : k;
+      if (q == me) mine = S;
+      S = through(S, m.cA[parity][q][lane], m.cH[parity][q][lane]);
+    }
+    entering = mine;
+    F s = mine;
+#pragma unroll
+    for (int k = 0; k < kWarps - 1; ++k) {
+      const int q = REVERSE ? kWarps - 1 - k : k;
+      if (REVERSE ? q > w : q < w) s = through(s, m.A[parity][q][lane], m.H[parity][q][lane]);
+    }
+    return s;
+  } else {
+    entering = S;
+    F mine = S;
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) {
+      const int q = REVERSE ? kWarps - 1 - k : k;
+      if (q == w) mine = S;
+      S = through(S, m.A[parity][q][lane], m.H[parity][q][lane]);
+    }
+    return mine;
   }
-  sigmoid2(g, q.s, q.c);
-  sigmoid2(beta, q.i, q.ci);
-  q.u = rate * q.s;
-  q.a = ex2(q.u * kLog2e);
-  q.m = sqrtf(one_minus_exp(-2.f * q.u, q.a * q.a));
-  if (reset) {
-    q.a = 0.f;
-    q.m = 1.f;
-  }
-  q.b = q.m * q.i * x;
-  return q;
 }
 
-template <typename T, typename G, bool LOGITS>
-__global__ void __launch_bounds__(128)
+// What a thread's place is: batch b, first channel c, rank and size of the cluster.
+struct Place {
+  int64_t b, c;
+  int rank, size;
+  bool on;  // the lane has a channel
+};
+template <int V, bool CLUSTER> __device__ __forceinline__ Place place(int64_t C) {
+  Place p;
+  p.rank = CLUSTER ? (int)cluster_rank() : 0;
+  p.size = CLUSTER ? (int)cluster_size() : 1;
+  const int64_t slabs = (C + 32 * V - 1) / (32 * V), i = blockIdx.x / p.size;
+  p.b = i / slabs;
+  p.c = (i % slabs) * (32 * V) + (threadIdx.x & 31) * V;
+  p.on = p.c < C;
+  return p;
+}
+
+// Bit i: the warp's step t0 + i is a reset (steps from L on are not).
+__device__ __forceinline__ uint32_t reset_bits(const uint8_t* reset, int64_t t0, int64_t L) {
+  const int lane = threadIdx.x & 31;
+  const bool r = lane < kSteps && t0 + lane < L && reset[t0 + lane] != 0;
+  return __ballot_sync(0xffffffffu, r);
+}
+
+// ---------------------------------------------------------------------------
+// Forward
+// ---------------------------------------------------------------------------
+template <typename T, typename G, int V> struct FwdRing {
+  uint8_t x[kStages][kWarps][kSteps][32 * Elem<T, V>::kBytes];
+  uint8_t g[kStages][kWarps][kSteps][32 * Elem<G, V>::kBytes];
+  uint8_t b[kStages][kWarps][kSteps][32 * Elem<G, V>::kBytes];
+};
+
+template <typename T, typename G, int V, bool LOGITS, bool RESET, bool CLUSTER>
+__global__ void __launch_bounds__(kThreads)
 glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __restrict__ beta,
                const float* __restrict__ decay, const float* __restrict__ h0,
                const uint8_t* __restrict__ reset, T* __restrict__ h, float* __restrict__ hT,
                float* __restrict__ ckpt, int64_t L, int64_t C, Strides st, float scale) {
-  const int64_t c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, b = blockIdx.y;
-  if (c >= C) return;
-  const float rate = LOGITS ? log_decay(decay[c], scale) : 0.f;
-  const int64_t nck = (L + kCkpt - 1) / kCkpt;
-  float s = h0 ? h0[b * C + c] : 0.f;
-  for (int64_t t = 0; t < L; ++t) {
-    if (ckpt && t % kCkpt == 0) ckpt[(b * nck + t / kCkpt) * C + c] = s;
-    const Gate q = gate_of<LOGITS>(to_f<T>(x[b * st.xb + t * st.xl + c]),
-                                   to_f<G>(g[b * st.gb + t * st.gl + c]),
-                                   to_f<G>(beta[b * st.bb + t * st.bl + c]), rate,
-                                   reset && reset[b * L + t]);
-    s = q.a == 0.f ? q.b : fmaf(q.a, s, q.b);
-    h[(b * L + t) * C + c] = from_f<T>(s);
+  using F = typename Lane<V>::F;
+  using EX = Elem<T, V>;
+  using EG = Elem<G, V>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  auto& ring = *reinterpret_cast<FwdRing<T, G, V>*>(smem);
+  __shared__ Maps<F, CLUSTER> maps;
+  const Place p = place<V, CLUSTER>(C);
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t tiles = (L + kTile - 1) / kTile, rounds = (tiles + p.size - 1) / p.size;
+  if (p.on) {
+    x += p.b * st.xb + p.c;
+    g += p.b * st.gb + p.c;
+    beta += p.b * st.bb + p.c;
+    h += p.b * L * C + p.c;
   }
-  if (hT) hT[b * C + c] = s;
+  if (RESET) reset += p.b * L;
+  F r1 = all_<F>(0.f), r2 = all_<F>(0.f);  // log2 a and -2 log a of an open gate
+  F S = all_<F>(0.f);
+  if (p.on) {
+    if (LOGITS) {
+      const F rate = map_([&](float d) { return scale * softplus(d); },
+                          Elem<float, V>::load(decay + p.c));
+      r1 = mul_(rate, all_<F>(-kLog2e));
+      r2 = mul_(rate, all_<F>(2.f));
+    }
+    if (h0) S = Elem<float, V>::load(h0 + p.b * C + p.c);
+  }
+  auto fetch = [&](int64_t round) {
+    const int64_t t0 = (round * p.size + p.rank) * kTile + w * kSteps;
+    const int s = (int)(round % kStages);
+    if (p.on && round < rounds) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        if (t0 + i < L) {
+          EX::copy(&ring.x[s][w][i][lane * EX::kBytes], x + (t0 + i) * st.xl);
+          EG::copy(&ring.g[s][w][i][lane * EG::kBytes], g + (t0 + i) * st.gl);
+          EG::copy(&ring.b[s][w][i][lane * EG::kBytes], beta + (t0 + i) * st.bl);
+        }
+      }
+    }
+    copy_commit();
+  };
+#pragma unroll
+  for (int k = 0; k < kStages - 1; ++k) fetch(k);
+  for (int64_t round = 0; round < rounds; ++round) {
+    const int64_t tile = round * p.size + p.rank, t0 = tile * kTile + w * kSteps;
+    const int n = t0 < L ? (int)(L - t0 < kSteps ? L - t0 : kSteps) : 0;
+    const int s = (int)(round % kStages);
+    fetch(round + kStages - 1);
+    const uint32_t rs = RESET ? reset_bits(reset, t0, L) : 0;
+    copy_wait<kStages - 1>();
+    F a[kSteps], b[kSteps], A = all_<F>(1.f), H = all_<F>(0.f);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const F xv = EX::load(&ring.x[s][w][i][lane * EX::kBytes]);
+      const F gv = EG::load(&ring.g[s][w][i][lane * EG::kBytes]);
+      const F bv = EG::load(&ring.b[s][w][i][lane * EG::kBytes]);
+      if (LOGITS) {
+        // 1 / (1 + e^-z): 0 and 1 at -inf and +inf
+        auto sig = [](float z) { return rcp(1.f + ex2(z)); };
+        const F sg = map_(sig, mul_(gv, all_<F>(-kLog2e)));
+        a[i] = map_([](float z) { return ex2(z); }, mul_(sg, r1));
+        F m = map_(sqrt_, one_minus_exp(mul_(sg, r2), mul_(a[i], a[i])));
+        if (RESET && (rs >> i & 1)) m = all_<F>(1.f);
+        b[i] = mul_(mul_(m, map_(sig, mul_(bv, all_<F>(-kLog2e)))), xv);
+      } else {
+        a[i] = gv;
+        b[i] = mul_(bv, xv);
+      }
+      if (RESET && (rs >> i & 1)) {
+        a[i] = all_<F>(0.f);
+        H = all_<F>(0.f);
+      }
+      if (i >= n) {  // behind the end: the state passes
+        a[i] = all_<F>(1.f);
+        b[i] = all_<F>(0.f);
+      }
+      A = mul_(A, a[i]);
+      H = fma_(a[i], H, b[i]);
+    }
+    F entering;
+    F hv = carry_in<F, CLUSTER, false>(maps, (int)(round & 1), A, H, S, entering);
+    if (p.on) {
+      if (ckpt && w == 0 && tile < tiles)
+        Elem<float, V>::store(ckpt + (p.b * tiles + tile) * C + p.c, entering);
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        if (RESET && (rs >> i & 1)) hv = all_<F>(0.f);
+        hv = fma_(a[i], hv, b[i]);
+        if (i < n) EX::store(h + (t0 + i) * C, hv);
+      }
+      // the warp that has the last step
+      if (hT && n > 0 && t0 + n == L) Elem<float, V>::store(hT + p.b * C + p.c, hv);
+    }
+    __syncwarp();
+  }
+  if (L == 0 && hT && p.on && w == 0) Elem<float, V>::store(hT + p.b * C + p.c, S);
+  copy_wait<0>();
 }
 
-template <typename T, typename G, bool LOGITS>
-__global__ void __launch_bounds__(128)
+// ---------------------------------------------------------------------------
+// Backward
+// ---------------------------------------------------------------------------
+template <typename T, typename G, int V> struct BwdRing {
+  FwdRing<T, G, V> in;
+  uint8_t d[kStages][kWarps][kSteps][32 * Elem<T, V>::kBytes];
+};
+
+template <typename T, typename G, int V, bool LOGITS, bool RESET, bool CLUSTER>
+__global__ void __launch_bounds__(kThreads, 2)
 glr_bwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __restrict__ beta,
                const float* __restrict__ decay, const uint8_t* __restrict__ reset,
                const float* __restrict__ ckpt, const T* __restrict__ dh,
                const float* __restrict__ dhT, T* __restrict__ dx, G* __restrict__ dg,
                G* __restrict__ dbeta, float* __restrict__ dh0, float* __restrict__ ddecay_part,
                int64_t L, int64_t C, Strides st, float scale) {
-  const int64_t c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, b = blockIdx.y;
-  if (c >= C) return;
-  const float rate = LOGITS ? log_decay(decay[c], scale) : 0.f;
-  const int64_t nck = (L + kCkpt - 1) / kCkpt;
-  float d = dhT ? dhT[b * C + c] : 0.f, sum = 0.f;
-  for (int64_t j = nck - 1; j >= 0; --j) {
-    float before[kCkpt];
-    float s = ckpt[(b * nck + j) * C + c];
-    const int64_t t0 = j * kCkpt;
-    const int n = (int)(L - t0 < kCkpt ? L - t0 : kCkpt);
-    auto gate = [&](int64_t t) {
-      return gate_of<LOGITS>(to_f<T>(x[b * st.xb + t * st.xl + c]),
-                             to_f<G>(g[b * st.gb + t * st.gl + c]),
-                             to_f<G>(beta[b * st.bb + t * st.bl + c]), rate,
-                             reset && reset[b * L + t]);
-    };
-    for (int k = 0; k < n; ++k) {
-      before[k] = s;
-      const Gate q = gate(t0 + k);
-      s = q.a == 0.f ? q.b : fmaf(q.a, s, q.b);
-    }
-    for (int k = n - 1; k >= 0; --k) {
-      const int64_t t = t0 + k, o = (b * L + t) * C + c;
-      const Gate q = gate(t);
-      const bool rs = reset && reset[b * L + t];
-      const float xv = to_f<T>(x[b * st.xb + t * st.xl + c]);
-      d += to_f<T>(dh[o]);
-      if (!LOGITS) {
-        dx[o] = from_f<T>(d * to_f<G>(beta[b * st.bb + t * st.bl + c]));
-        dg[o] = from_f<G>(rs ? 0.f : d * before[k]);
-        dbeta[o] = from_f<G>(d * xv);
-      } else {
-        // a^2 / m -> the gradient's limit is 0 where a == 1 (m == 0)
-        const float am = q.m > 0.f ? q.a / q.m : 0.f;
-        const float du = rs ? 0.f : d * q.a * (before[k] - am * q.i * xv);
-        sum = fmaf(du, q.s, sum);
-        dg[o] = from_f<G>(du * q.u * q.c);
-        const float dm = d * q.m;
-        dx[o] = from_f<T>(dm * q.i);
-        dbeta[o] = from_f<G>(dm * xv * q.i * q.ci);
+  using F = typename Lane<V>::F;
+  using EX = Elem<T, V>;
+  using EG = Elem<G, V>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  auto& ring = *reinterpret_cast<BwdRing<T, G, V>*>(smem);
+  __shared__ Maps<F, false> fwd_maps;
+  __shared__ Maps<F, CLUSTER> maps;
+  const Place p = place<V, CLUSTER>(C);
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t tiles = (L + kTile - 1) / kTile, rounds = (tiles + p.size - 1) / p.size;
+  if (p.on) {
+    x += p.b * st.xb + p.c;
+    g += p.b * st.gb + p.c;
+    beta += p.b * st.bb + p.c;
+    dh += p.b * L * C + p.c;
+    dx += p.b * L * C + p.c;
+    dg += p.b * L * C + p.c;
+    dbeta += p.b * L * C + p.c;
+  }
+  if (RESET) reset += p.b * L;
+  F rate = all_<F>(0.f), sum = all_<F>(0.f);
+  F R = all_<F>(0.f);  // a_t D_t of the step behind the round
+  if (p.on) {
+    if (LOGITS)
+      rate = map_([&](float d) { return -scale * softplus(d); }, Elem<float, V>::load(decay + p.c));
+    if (dhT) R = Elem<float, V>::load(dhT + p.b * C + p.c);
+  }
+  auto fetch = [&](int64_t k) {  // k-th round from the end
+    const int64_t t0 = ((rounds - 1 - k) * p.size + p.rank) * kTile + w * kSteps;
+    const int s = (int)(k % kStages);
+    if (p.on && k < rounds) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        if (t0 + i < L) {
+          EX::copy(&ring.in.x[s][w][i][lane * EX::kBytes], x + (t0 + i) * st.xl);
+          EG::copy(&ring.in.g[s][w][i][lane * EG::kBytes], g + (t0 + i) * st.gl);
+          EG::copy(&ring.in.b[s][w][i][lane * EG::kBytes], beta + (t0 + i) * st.bl);
+          EX::copy(&ring.d[s][w][i][lane * EX::kBytes], dh + (t0 + i) * C);
+        }
       }
-      d = q.a == 0.f ? 0.f : q.a * d;
+    }
+    copy_commit();
+  };
+#pragma unroll
+  for (int k = 0; k < kStages - 1; ++k) fetch(k);
+  for (int64_t k = 0; k < rounds; ++k) {
+    const int64_t tile = (rounds - 1 - k) * p.size + p.rank, t0 = tile * kTile + w * kSteps;
+    const int n = t0 < L ? (int)(L - t0 < kSteps ? L - t0 : kSteps) : 0;
+    const int s = (int)(k % kStages);
+    F first = all_<F>(0.f);  // the state in front of the tile
+    if (p.on && tile < tiles) first = Elem<float, V>::load(ckpt + (p.b * tiles + tile) * C + p.c);
+    fetch(k + kStages - 1);
+    const uint32_t rs = RESET ? reset_bits(reset, t0, L) : 0;
+    copy_wait<kStages - 1>();
+    // The gates of the steps.  lo_g, lo_b: the smaller of sigmoid and 1 - sigmoid, with the
+    // logit's sign, from which both follow without cancellation (values: beta and x).
+    F a[kSteps], m[kSteps], lo_g[kSteps], lo_b[kSteps], xv[kSteps], dv[kSteps];
+    F A = all_<F>(1.f), H = all_<F>(0.f), Q = all_<F>(0.f);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      xv[i] = EX::load(&ring.in.x[s][w][i][lane * EX::kBytes]);
+      dv[i] = EX::load(&ring.d[s][w][i][lane * EX::kBytes]);
+      const F gv = EG::load(&ring.in.g[s][w][i][lane * EG::kBytes]);
+      const F bv = EG::load(&ring.in.b[s][w][i][lane * EG::kBytes]);
+      F b;
+      if (LOGITS) {
+        auto lower = [](float z) {
+          const float t = ex2(-fabsf(z) * kLog2e);
+          return copysignf(t * rcp(1.f + t), z);
+        };
+        // sigmoid from the smaller part
+        auto sig = [](float l) { return signbit(l) ? -l : 1.f - l; };
+        lo_g[i] = map_(lower, gv);
+        lo_b[i] = map_(lower, bv);
+        const F u = mul_(rate, map_(sig, lo_g[i]));
+        a[i] = map_([](float z) { return ex2(z * kLog2e); }, u);
+        m[i] = map_(sqrt_, one_minus_exp(mul_(u, all_<F>(-2.f)), mul_(a[i], a[i])));
+        if (RESET && (rs >> i & 1)) m[i] = all_<F>(1.f);
+        b = mul_(mul_(m[i], map_(sig, lo_b[i])), xv[i]);
+      } else {
+        a[i] = gv;
+        lo_b[i] = bv;
+        b = mul_(bv, xv[i]);
+      }
+      if (RESET && (rs >> i & 1)) {
+        a[i] = all_<F>(0.f);
+        H = all_<F>(0.f);
+      }
+      if (i >= n) {
+        a[i] = all_<F>(1.f);
+        xv[i] = b = dv[i] = all_<F>(0.f);
+      }
+      A = mul_(A, a[i]);
+      H = fma_(a[i], H, b);
+    }
+#pragma unroll
+    for (int i = kSteps - 1; i >= 0; --i) {  // Q: D of step i, without what enters
+      if (i + 1 < kSteps) Q = RESET && (rs >> (i + 1) & 1) ? dv[i] : fma_(a[i + 1], Q, dv[i]);
+      else Q = dv[i];
+    }
+    Q = RESET && (rs & 1) ? all_<F>(0.f) : mul_(a[0], Q);
+    F unused;
+    F hv = carry_in<F, false, false>(fwd_maps, (int)(k & 1), A, H, first, unused);
+    F d = carry_in<F, CLUSTER, true>(maps, (int)(k & 1), A, Q, R, unused);
+    if (p.on) {
+    F before[kSteps];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      before[i] = hv;
+      F b;
+      if (LOGITS)
+        b = mul_(mul_(m[i], map_([](float l) { return signbit(l) ? -l : 1.f - l; }, lo_b[i])), xv[i]);
+      else
+        b = mul_(lo_b[i], xv[i]);
+      if (RESET && (rs >> i & 1)) hv = all_<F>(0.f);
+      hv = fma_(a[i], hv, b);
+    }
+#pragma unroll
+    for (int i = kSteps - 1; i >= 0; --i) {
+      const bool zero = RESET && (rs >> i & 1);
+      if (i + 1 == kSteps) d = add_(d, dv[i]);
+      else d = RESET && (rs >> (i + 1) & 1) ? dv[i] : fma_(a[i + 1], d, dv[i]);
+      F ox, og, ob;
+      if (LOGITS) {
+        auto small = [](float l) { return signbit(l) ? -l : 1.f - l; };
+        auto large = [](float l) { return signbit(l) ? 1.f + l : l; };  // 1 - sigmoid
+        const F u = mul_(rate, map_(small, lo_g[i]));
+        const F mi = mul_(m[i], map_(small, lo_b[i])), b = mul_(mi, xv[i]);
+        // a^2 / (1 - a^2); a == 1 leaves the limit 0 of (that * u * b)
+        const F q = map_([](float m_, float a_) { return m_ > 1e-18f ? a_ * a_ * rcp(m_ * m_) : 0.f; },
+                         m[i], a[i]);
+        F du = mul_(d, fma_(a[i], before[i], mul_(mul_(q, b), all_<F>(-1.f))));
+        if (zero) du = all_<F>(0.f);
+        if (i < n) sum = fma_(du, u, sum);
+        og = mul_(mul_(du, u), map_(large, lo_g[i]));
+        ox = mul_(d, mi);
+        ob = mul_(mul_(d, b), map_(large, lo_b[i]));
+      } else {
+        ox = mul_(d, lo_b[i]);
+        ob = mul_(d, xv[i]);
+        og = zero ? all_<F>(0.f) : mul_(d, before[i]);
+      }
+      if (i < n) {
+        const int64_t o = (t0 + i) * C;
+        EX::store(dx + o, ox);
+        EG::store(dg + o, og);
+        EG::store(dbeta + o, ob);
+      }
+    }
+    }
+    __syncwarp();
+  }
+  copy_wait<0>();
+  if (dh0 && p.on && p.rank == 0 && w == 0) Elem<float, V>::store(dh0 + p.b * C + p.c, R);
+  if (LOGITS && ddecay_part) {
+    __syncthreads();
+    fwd_maps.A[0][w][lane] = sum;
+    __syncthreads();
+    if (w == 0 && p.on) {
+      F t = fwd_maps.A[0][0][lane];
+#pragma unroll
+      for (int k = 1; k < kWarps; ++k) t = add_(t, fwd_maps.A[0][k][lane]);
+      Elem<float, V>::store(ddecay_part + (p.b * p.size + p.rank) * C + p.c, t);
     }
   }
-  if (dh0) dh0[b * C + c] = d;
-  if (ddecay_part) ddecay_part[b * C + c] = sum;
 }
 
-// ddecay[c] = -scale sigmoid(decay[c]) * the sum of the partial rows, in their order.
+// ddecay[c] = sigmoid(decay) / softplus(decay) * the sum of the partial rows of du u, in their
+// order: u = rate s and rate = -scale softplus, so -scale sigmoid(decay) du s is that.  The
+// quotient goes to 1 where softplus leaves the fp32 range.
 __global__ void __launch_bounds__(128)
 glr_ddecay_kernel(const float* __restrict__ part, int64_t rows, const float* __restrict__ decay,
-                  float* __restrict__ ddecay, int64_t C, float scale) {
+                  float* __restrict__ ddecay, int64_t C) {
   const int64_t c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (c >= C) return;
   float t = 0.f;
   for (int64_t r = 0; r < rows; ++r) t += part[r * C + c];
   float s, cs;
   sigmoid2(decay[c], s, cs);
-  ddecay[c] = -scale * s * t;
+  const float sp = softplus(decay[c]);
+  ddecay[c] = t * (sp > 1e-30f ? s / sp : 1.f);
 }
 
+// ---------------------------------------------------------------------------
+// One step
+// ---------------------------------------------------------------------------
 template <typename T, typename G, bool LOGITS>
 __global__ void __launch_bounds__(128)
 glr_step_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __restrict__ beta,
@@ -172,16 +566,26 @@ glr_step_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __res
                 int64_t B, int64_t C, Strides st, float scale) {
   const int64_t c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (c >= C) return;
-  const float rate = LOGITS ? log_decay(decay[c], scale) : 0.f;
+  const float rate = LOGITS ? -scale * softplus(decay[c]) : 0.f;
   for (int64_t b = blockIdx.y; b < B; b += gridDim.y) {
-    const Gate q = gate_of<LOGITS>(to_f<T>(x[b * st.xb + c]), to_f<G>(g[b * st.gb + c]),
-                                   to_f<G>(beta[b * st.bb + c]), rate, false);
-    const float s = q.a == 0.f ? q.b : fmaf(q.a, state[b * C + c], q.b);
+    float a = to_f<G>(g[b * st.gb + c]), in = to_f<G>(beta[b * st.bb + c]);
+    if (LOGITS) {
+      float s, i, unused;
+      sigmoid2(a, s, unused);
+      sigmoid2(in, i, unused);
+      const float u = rate * s;
+      a = ex2(u * kLog2e);
+      in = sqrt_(one_minus_exp(-2.f * u, a * a)) * i;
+    }
+    const float s = fmaf(a, state[b * C + c], in * to_f<T>(x[b * st.xb + c]));
     state[b * C + c] = s;
     h[b * C + c] = from_f<T>(s);
   }
 }
 
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
 // Calls f with values of the two element types of (dtype, gate_dtype): x's, and the gates',
 // which are x's or fp32.
 template <typename F>
@@ -202,13 +606,81 @@ int with_types(int dtype, int gate_dtype, F&& f) {
   return FO_EDTYPE;
 }
 
-int check_sizes(const char* what, int64_t B, int64_t L, int64_t C, int64_t most_b = 65535) {
+// Calls f with two integral constants: v == 1 or 2, and three truth values.
+template <typename F>
+int with_flags(bool two, bool logits, bool reset, bool cluster, F&& f) {
+  auto b = [](bool v, auto&& k) {
+    return v ? k(std::true_type{}) : k(std::false_type{});
+  };
+  return b(two, [&](auto t) {
+    return b(logits, [&](auto l) {
+      return b(reset, [&](auto r) { return b(cluster, [&](auto c) { return f(t, l, r, c); }); });
+    });
+  });
+}
+
+int check_sizes(const char* what, int64_t B, int64_t L, int64_t C) {
   FO_CHECK_ARG(B >= 0 && L >= 0 && C >= 0, "%s: negative size B=%lld L=%lld C=%lld", what,
                (long long)B, (long long)L, (long long)C);
-  FO_CHECK_ARG(B <= most_b, "%s: B=%lld is over 65535", what, (long long)B);
-  FO_CHECK_ARG(C <= (int64_t)1 << 31, "%s: C=%lld is over 2^31", what, (long long)C);
+  FO_CHECK_ARG(C == 0 || B <= ((int64_t)1 << 31) / 8 / ((C + 31) / 32),
+               "%s: B=%lld sequences of %lld channels are over the grid's limit", what,
+               (long long)B, (long long)C);
   return FO_OK;
 }
+
+bool multiple(const void* p, int64_t bytes) {
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0;
+}
+
+// Two channels a lane: pairs have to start at a multiple of their size everywhere.
+bool pairs_ok(const void* const* xs, int nx, const void* const* gs, int ng, const void* const* fs,
+              int nf, const int64_t* strides, int64_t C, int xbytes, int gbytes) {
+  bool ok = C % 2 == 0;
+  for (int i = 0; i < nx; ++i) ok = ok && multiple(xs[i], 2 * xbytes);
+  for (int i = 0; i < ng; ++i) ok = ok && multiple(gs[i], 2 * gbytes);
+  for (int i = 0; i < nf; ++i) ok = ok && multiple(fs[i], 8);
+  for (int i = 0; i < 6; ++i) ok = ok && strides[i] % 2 == 0;
+  return ok;
+}
+
+// CTAs of a cluster along time: doubled, up to 8 and up to the number of tiles, until there are
+// `want` CTAs.
+int cluster_for(int64_t ctas, int64_t L, int64_t want) {
+  const int64_t tiles = (L + kTile - 1) / kTile;
+  int n = 1;
+  while (n < 8 && ctas * n < want && 2 * n <= tiles) n *= 2;
+  return n;
+}
+
+template <typename K, typename... Args>
+int launch(const char* what, K kernel, int64_t ctas, int cluster, int smem, cudaStream_t st,
+           Args... args) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(ctas * cluster));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  }
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    set_error("%s: %s", what, cudaGetErrorString(e));
+    return FO_ECUDA;
+  }
+  return check_launch(what);
+}
+
+constexpr int64_t kZeroStrides[6] = {};
+
+int64_t slabs_of(int64_t C, int v) { return (C + 32 * v - 1) / (32 * v); }
 
 }  // namespace
 }  // namespace fo
@@ -223,19 +695,21 @@ extern "C" int fo_glr_fwd(const void* x, const void* g, const void* beta, const 
   if (int rc = check_sizes("gated recurrence", B, L, C)) return rc;
   if (B == 0 || C == 0) return FO_OK;
   FO_CHECK_ARG(L == 0 || (x && g && beta && h && strides), "gated recurrence: null pointer");
-  const Strides s = strides ? Strides{strides[0], strides[1], strides[2], strides[3], strides[4],
-                                      strides[5]}
-                            : Strides{};
+  const int64_t* q = strides ? strides : kZeroStrides;
+  const Strides s{q[0], q[1], q[2], q[3], q[4], q[5]};
   return with_types(dtype, gate_dtype, [&](auto t, auto gt) {
     using T = decltype(t);
     using G = decltype(gt);
-    auto run = [&](auto k) {
-      k<<<dim3((unsigned)((C + 127) / 128), (unsigned)B), 128, 0, as_stream(stream)>>>(
-          (const T*)x, (const G*)g, (const G*)beta, decay, h0, reset, (T*)h, hT, ckpt, L, C, s,
-          scale);
-      return check_launch("glr_fwd_kernel");
-    };
-    return decay ? run(glr_fwd_kernel<T, G, true>) : run(glr_fwd_kernel<T, G, false>);
+    const void *xs[] = {x, h}, *gs[] = {g, beta}, *fs[] = {decay, h0, hT, ckpt};
+    const bool two = pairs_ok(xs, 2, gs, 2, fs, 4, q, C, sizeof(T), sizeof(G));
+    const int64_t ctas = B * slabs_of(C, two ? 2 : 1);
+    const int cl = cluster_for(ctas, L, 2 * num_sms());
+    return with_flags(two, decay, reset, cl > 1, [&](auto tw, auto lo, auto rs, auto c) {
+      constexpr int V = tw ? 2 : 1;
+      return launch("glr_fwd_kernel", glr_fwd_kernel<T, G, V, lo, rs, c>, ctas, cl,
+                    (int)sizeof(FwdRing<T, G, V>), as_stream(stream), (const T*)x, (const G*)g,
+                    (const G*)beta, decay, h0, reset, (T*)h, hT, ckpt, L, C, s, scale);
+    });
   });
 }
 
@@ -243,7 +717,7 @@ extern "C" int fo_glr_step(const void* x, const void* g, const void* beta, const
                            float* state, void* h, int64_t B, int64_t C, const int64_t* strides,
                            float scale, int dtype, int gate_dtype, void* stream) {
   clear_error();
-  if (int rc = check_sizes("gated recurrence step", B, 1, C, INT64_MAX)) return rc;
+  if (int rc = check_sizes("gated recurrence step", B, 1, C)) return rc;
   if (B == 0 || C == 0) return FO_OK;
   FO_CHECK_ARG(x && g && beta && state && h && strides, "gated recurrence step: null pointer");
   const Strides s{strides[0], 0, strides[1], 0, strides[2], 0};
@@ -251,8 +725,9 @@ extern "C" int fo_glr_step(const void* x, const void* g, const void* beta, const
     using T = decltype(t);
     using G = decltype(gt);
     auto run = [&](auto k) {
-      k<<<dim3((unsigned)((C + 127) / 128), (unsigned)(B < 65535 ? B : 65535)), 128, 0, as_stream(stream)>>>(
-          (const T*)x, (const G*)g, (const G*)beta, decay, state, (T*)h, B, C, s, scale);
+      k<<<dim3((unsigned)((C + 127) / 128), (unsigned)(B < 65535 ? B : 65535)), 128, 0,
+          as_stream(stream)>>>((const T*)x, (const G*)g, (const G*)beta, decay, state, (T*)h, B, C,
+                               s, scale);
       return check_launch("glr_step_kernel");
     };
     return decay ? run(glr_step_kernel<T, G, true>) : run(glr_step_kernel<T, G, false>);
@@ -263,7 +738,7 @@ extern "C" int fo_glr_bwd_workspace_bytes(int64_t B, int64_t L, int64_t C, int64
   clear_error();
   FO_CHECK_ARG(bytes, "gated recurrence backward: null pointer");
   if (int rc = check_sizes("gated recurrence backward", B, L, C)) return rc;
-  *bytes = B * C * 4;
+  *bytes = B * 8 * C * 4;
   return FO_OK;
 }
 
@@ -290,23 +765,27 @@ extern "C" int fo_glr_bwd(const void* x, const void* g, const void* beta, const 
     set_error("gated recurrence backward: workspace of %lld bytes required", (long long)need);
     return FO_EWORKSPACE;
   }
-  const Strides s = strides ? Strides{strides[0], strides[1], strides[2], strides[3], strides[4],
-                                      strides[5]}
-                            : Strides{};
+  FO_CHECK_ARG(!need || multiple(workspace, 8),
+               "gated recurrence backward: workspace must be 8-byte aligned");
+  const int64_t* sq = strides ? strides : kZeroStrides;
+  const Strides s{sq[0], sq[1], sq[2], sq[3], sq[4], sq[5]};
   float* part = ddecay ? (float*)workspace : nullptr;
   return with_types(dtype, gate_dtype, [&](auto t, auto gt) {
     using T = decltype(t);
     using G = decltype(gt);
-    auto run = [&](auto k) {
-      k<<<dim3((unsigned)((C + 127) / 128), (unsigned)B), 128, 0, q>>>(
-          (const T*)x, (const G*)g, (const G*)beta, decay, reset, ckpt, (const T*)dh, dhT, (T*)dx,
-          (G*)dg, (G*)dbeta, dh0, part, L, C, s, scale);
-      return check_launch("glr_bwd_kernel");
-    };
-    int rc = decay ? run(glr_bwd_kernel<T, G, true>) : run(glr_bwd_kernel<T, G, false>);
+    const void *xs[] = {x, dh, dx}, *gs[] = {g, beta, dg, dbeta}, *fs[] = {decay, ckpt, dhT, dh0};
+    const bool two = pairs_ok(xs, 3, gs, 4, fs, 4, sq, C, sizeof(T), sizeof(G));
+    const int64_t ctas = B * slabs_of(C, two ? 2 : 1);
+    const int cl = cluster_for(ctas, L, 2 * num_sms());
+    int rc = with_flags(two, decay, reset, cl > 1, [&](auto tw, auto lo, auto rs, auto c) {
+      constexpr int V = tw ? 2 : 1;
+      return launch("glr_bwd_kernel", glr_bwd_kernel<T, G, V, lo, rs, c>, ctas, cl,
+                    (int)sizeof(BwdRing<T, G, V>), q, (const T*)x, (const G*)g, (const G*)beta,
+                    decay, reset, ckpt, (const T*)dh, dhT, (T*)dx, (G*)dg, (G*)dbeta, dh0, part,
+                    L, C, s, scale);
+    });
     if (rc || !ddecay) return rc;
-    glr_ddecay_kernel<<<(unsigned)((C + 127) / 128), 128, 0, q>>>(part, B, decay, ddecay, C,
-                                                                  scale);
+    glr_ddecay_kernel<<<(unsigned)((C + 127) / 128), 128, 0, q>>>(part, B * cl, decay, ddecay, C);
     return check_launch("glr_ddecay_kernel");
   });
 }

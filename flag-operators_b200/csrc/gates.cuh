@@ -26,4 +26,55 @@ __device__ __forceinline__ void sigmoid2(float z, float& s, float& c) {
   c = z < 0.f ? hi : lo;
 }
 
+// ---------------------------------------------------------------------------
+// One or two fp32 values handled alike: float, or float2 with the packed instructions (two
+// results per issue slot).
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ float fma_(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float mul_(float a, float b) { return a * b; }
+__device__ __forceinline__ float add_(float a, float b) { return a + b; }
+__device__ __forceinline__ float2 fma_(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)),
+        "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 mul_(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 add_(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+template <typename F> __device__ __forceinline__ F all_(float x);
+template <> __device__ __forceinline__ float all_<float>(float x) { return x; }
+template <> __device__ __forceinline__ float2 all_<float2>(float x) { return make_float2(x, x); }
+// f on every value
+template <typename Fn> __device__ __forceinline__ float map_(Fn f, float a) { return f(a); }
+template <typename Fn> __device__ __forceinline__ float2 map_(Fn f, float2 a) {
+  return make_float2(f(a.x), f(a.y));
+}
+template <typename Fn> __device__ __forceinline__ float map_(Fn f, float a, float b) {
+  return f(a, b);
+}
+template <typename Fn> __device__ __forceinline__ float2 map_(Fn f, float2 a, float2 b) {
+  return make_float2(f(a.x, b.x), f(a.y, b.y));
+}
+template <typename Fn> __device__ __forceinline__ float map_(Fn f, float a, float b, float c) {
+  return f(a, b, c);
+}
+template <typename Fn>
+__device__ __forceinline__ float2 map_(Fn f, float2 a, float2 b, float2 c) {
+  return make_float2(f(a.x, b.x, c.x), f(a.y, b.y, c.y));
+}
+
 }  // namespace fo
