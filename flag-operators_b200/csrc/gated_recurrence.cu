@@ -68,13 +68,15 @@ __device__ __forceinline__ float softplus(float decay) {
   return decay > 20.f ? decay : log1pf(expf(decay));
 }
 
-// The state s behind a segment that maps it to A s + H.  A zero on either side leaves H, so that an
-// A that left the fp32 range over an empty state, or a state before a reset, adds nothing.
-__device__ __forceinline__ float through1(float s, float A, float H) {
-  return s == 0.f || A == 0.f ? H : fmaf(A, s, H);
+// The state s behind a segment that maps it to A s + H.  Where a segment may hold a reset (A is 0),
+// what is in front of it is not looked at, not even a NaN.
+template <bool RESET, typename F> __device__ __forceinline__ F through(F s, F A, F H) {
+  if (RESET) return map_([](float s_, float a, float h) { return a == 0.f ? h : fmaf(a, s_, h); }, s, A, H);
+  return fma_(A, s, H);
 }
-template <typename F> __device__ __forceinline__ F through(F s, F A, F H) {
-  return map_(through1, s, A, H);
+// A product of gates above 1 may leave the fp32 range over a state of zero: kept finite, it adds 0.
+template <typename F> __device__ __forceinline__ F finite(F A) {
+  return map_([](float a) { return fminf(fmaxf(a, -3.4028235e38f), 3.4028235e38f); }, A);
 }
 
 // ---------------------------------------------------------------------------
@@ -110,6 +112,7 @@ template <typename T, int V> struct Elem {
     }
     *reinterpret_cast<W*>(p) = w;
   }
+  static __device__ __forceinline__ void zero(void* smem) { *reinterpret_cast<W*>(smem) = W{}; }
   // global -> shared without waiting (2-byte elements have no such copy: through a register)
   static __device__ __forceinline__ void copy(void* smem, const T* p) {
     if constexpr (kBytes == 2) {
@@ -122,6 +125,33 @@ template <typename T, int V> struct Elem {
     }
   }
 };
+// A warp's kSteps rows of a stream into its part of the ring; lanes without a channel and rows from
+// `rows` on are left out.  wide: 16 bytes a copy, rows shared out over the lanes (so a __syncwarp
+// has to follow the wait); otherwise every lane copies just its own elements.
+template <typename T, int V>
+__device__ __forceinline__ void copy_rows(uint8_t (*ring)[32 * Elem<T, V>::kBytes], const T* row0,
+                                          int64_t step, int64_t C_left, int rows, bool wide) {
+  using E = Elem<T, V>;
+  const int lane = threadIdx.x & 31;
+  if (wide) {
+    constexpr int kPer = 16 / (int)sizeof(T);         // elements of a copy
+    constexpr int kRow = 32 * V / kPer;               // copies of a row
+#pragma unroll
+    for (int k = 0; k < (kSteps * kRow) / 32; ++k) {
+      const int r = (k * 32 + lane) / kRow, c = (lane % kRow) * kPer;
+      if (r < rows && c < C_left)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                         (uint32_t)__cvta_generic_to_shared(&ring[r][c * (int)sizeof(T)])),
+                     "l"(row0 + r * step + c)
+                     : "memory");
+    }
+  } else if (lane * V < C_left) {
+    const T* p = row0 + lane * V;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i, p += step)
+      if (i < rows) E::copy(&ring[i][lane * E::kBytes], p);
+  }
+}
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
@@ -169,10 +199,10 @@ template <typename F, bool CLUSTER> struct Maps {
 // From this warp's map (A, H) and the state S in front of the round: the state in front of
 // this warp's steps; S becomes the state behind the round.  REVERSE walks the warps and CTAs from
 // the last to the first.  entering: the state in front of the CTA's tile.
-template <typename F, bool CLUSTER, bool REVERSE>
+template <typename F, bool CLUSTER, bool REVERSE, bool RESET>
 __device__ __forceinline__ F carry_in(Maps<F, CLUSTER>& m, int parity, F A, F H, F& S, F& entering) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  m.A[parity][w][lane] = A;
+  m.A[parity][w][lane] = finite(A);
   m.H[parity][w][lane] = H;
   __syncthreads();
   if constexpr (CLUSTER) {
@@ -183,9 +213,8 @@ __device__ __forceinline__ F carry_in(Maps<F, CLUSTER>& m, int parity, F A, F H,
       for (int k = 0; k < kWarps; ++k) {
         const int q = REVERSE ? kWarps - 1 - k : k;
         const F ak = m.A[parity][q][lane];
-        h = through(h, ak, m.H[parity][q][lane]);
-        // 0 once any factor is 0, whatever the others are
-        a = map_([](float x, float y) { return x == 0.f || y == 0.f ? 0.f : x * y; }, a, ak);
+        h = through<RESET>(h, ak, m.H[parity][q][lane]);
+        a = finite(mul_(a, ak));
       }
       store_remote(&m.cA[parity][me][lane], w, a);
       store_remote(&m.cH[parity][me][lane], w, h);
@@ -195,24 +224,24 @@ __device__ __forceinline__ F carry_in(Maps<F, CLUSTER>& m, int parity, F A, F H,
     for (uint32_t k = 0; k < n; ++k) {
       const uint32_t q = REVERSE ? n - 1 - k : k;
       if (q == me) mine = S;
-      S = through(S, m.cA[parity][q][lane], m.cH[parity][q][lane]);
+      S = through<RESET>(S, m.cA[parity][q][lane], m.cH[parity][q][lane]);
     }
     entering = mine;
     F s = mine;
 #pragma unroll
     for (int k = 0; k < kWarps - 1; ++k) {
       const int q = REVERSE ? kWarps - 1 - k : k;
-      if (REVERSE ? q > w : q < w) s = through(s, m.A[parity][q][lane], m.H[parity][q][lane]);
+      if (REVERSE ? q > w : q < w) s = through<RESET>(s, m.A[parity][q][lane], m.H[parity][q][lane]);
     }
     return s;
   } else {
     entering = S;
     F mine = S;
-#pragma unroll
+#pragma unroll 4  // more would hold the maps of all warps in registers at once
     for (int k = 0; k < kWarps; ++k) {
       const int q = REVERSE ? kWarps - 1 - k : k;
       if (q == w) mine = S;
-      S = through(S, m.A[parity][q][lane], m.H[parity][q][lane]);
+      S = through<RESET>(S, m.A[parity][q][lane], m.H[parity][q][lane]);
     }
     return mine;
   }
@@ -220,7 +249,7 @@ __device__ __forceinline__ F carry_in(Maps<F, CLUSTER>& m, int parity, F A, F H,
 
 // What a thread's place is: batch b, first channel c, rank and size of the cluster.
 struct Place {
-  int64_t b, c;
+  int64_t b, c0, c;  // c0: the slab's first channel
   int rank, size;
   bool on;  // the lane has a channel
 };
@@ -230,7 +259,8 @@ template <int V, bool CLUSTER> __device__ __forceinline__ Place place(int64_t C)
   p.size = CLUSTER ? (int)cluster_size() : 1;
   const int64_t slabs = (C + 32 * V - 1) / (32 * V), i = blockIdx.x / p.size;
   p.b = i / slabs;
-  p.c = (i % slabs) * (32 * V) + (threadIdx.x & 31) * V;
+  p.c0 = (i % slabs) * (32 * V);
+  p.c = p.c0 + (threadIdx.x & 31) * V;
   p.on = p.c < C;
   return p;
 }
@@ -256,7 +286,7 @@ __global__ void __launch_bounds__(kThreads)
 glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __restrict__ beta,
                const float* __restrict__ decay, const float* __restrict__ h0,
                const uint8_t* __restrict__ reset, T* __restrict__ h, float* __restrict__ hT,
-               float* __restrict__ ckpt, int64_t L, int64_t C, Strides st, float scale) {
+               float* __restrict__ ckpt, int64_t L, int64_t C, Strides st, float scale, bool wide) {
   using F = typename Lane<V>::F;
   using EX = Elem<T, V>;
   using EG = Elem<G, V>;
@@ -266,12 +296,9 @@ glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
   const Place p = place<V, CLUSTER>(C);
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t tiles = (L + kTile - 1) / kTile, rounds = (tiles + p.size - 1) / p.size;
-  if (p.on) {
-    x += p.b * st.xb + p.c;
-    g += p.b * st.gb + p.c;
-    beta += p.b * st.bb + p.c;
-    h += p.b * L * C + p.c;
-  }
+  x += p.b * st.xb + p.c0;
+  g += p.b * st.gb + p.c0;
+  beta += p.b * st.bb + p.c0;
   if (RESET) reset += p.b * L;
   F r1 = all_<F>(0.f), r2 = all_<F>(0.f);  // log2 a and -2 log a of an open gate
   F S = all_<F>(0.f);
@@ -284,18 +311,14 @@ glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
     }
     if (h0) S = Elem<float, V>::load(h0 + p.b * C + p.c);
   }
+  auto rows_of = [&](int64_t t0) { return t0 < L ? (int)(L - t0 < kSteps ? L - t0 : kSteps) : 0; };
   auto fetch = [&](int64_t round) {
     const int64_t t0 = (round * p.size + p.rank) * kTile + w * kSteps;
-    const int s = (int)(round % kStages);
-    if (p.on && round < rounds) {
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        if (t0 + i < L) {
-          EX::copy(&ring.x[s][w][i][lane * EX::kBytes], x + (t0 + i) * st.xl);
-          EG::copy(&ring.g[s][w][i][lane * EG::kBytes], g + (t0 + i) * st.gl);
-          EG::copy(&ring.b[s][w][i][lane * EG::kBytes], beta + (t0 + i) * st.bl);
-        }
-      }
+    const int s = (int)(round % kStages), n = rows_of(t0);
+    if (n > 0) {
+      copy_rows<T, V>(ring.x[s][w], x + t0 * st.xl, st.xl, C - p.c0, n, wide);
+      copy_rows<G, V>(ring.g[s][w], g + t0 * st.gl, st.gl, C - p.c0, n, wide);
+      copy_rows<G, V>(ring.b[s][w], beta + t0 * st.bl, st.bl, C - p.c0, n, wide);
     }
     copy_commit();
   };
@@ -303,11 +326,11 @@ glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
   for (int k = 0; k < kStages - 1; ++k) fetch(k);
   for (int64_t round = 0; round < rounds; ++round) {
     const int64_t tile = round * p.size + p.rank, t0 = tile * kTile + w * kSteps;
-    const int n = t0 < L ? (int)(L - t0 < kSteps ? L - t0 : kSteps) : 0;
-    const int s = (int)(round % kStages);
+    const int n = rows_of(t0), s = (int)(round % kStages);
     fetch(round + kStages - 1);
     const uint32_t rs = RESET ? reset_bits(reset, t0, L) : 0;
     copy_wait<kStages - 1>();
+    __syncwarp();
     F a[kSteps], b[kSteps], A = all_<F>(1.f), H = all_<F>(0.f);
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
@@ -316,38 +339,51 @@ glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
       const F bv = EG::load(&ring.b[s][w][i][lane * EG::kBytes]);
       if (LOGITS) {
         // 1 / (1 + e^-z): 0 and 1 at -inf and +inf
-        auto sig = [](float z) { return rcp(1.f + ex2(z)); };
-        const F sg = map_(sig, mul_(gv, all_<F>(-kLog2e)));
-        a[i] = map_([](float z) { return ex2(z); }, mul_(sg, r1));
+        auto sig = [](F z) {
+          const F e = map_(ex2, mul_(z, all_<F>(-kLog2e)));
+          return map_(rcp, add_(e, all_<F>(1.f)));
+        };
+        const F sg = sig(gv);
+        a[i] = map_(ex2, mul_(sg, r1));
         F m = map_(sqrt_, one_minus_exp(mul_(sg, r2), mul_(a[i], a[i])));
         if (RESET && (rs >> i & 1)) m = all_<F>(1.f);
-        b[i] = mul_(mul_(m, map_(sig, mul_(bv, all_<F>(-kLog2e)))), xv);
+        b[i] = mul_(mul_(m, sig(bv)), xv);
       } else {
         a[i] = gv;
         b[i] = mul_(bv, xv);
       }
-      if (RESET && (rs >> i & 1)) {
-        a[i] = all_<F>(0.f);
-        H = all_<F>(0.f);
-      }
-      if (i >= n) {  // behind the end: the state passes
-        a[i] = all_<F>(1.f);
-        b[i] = all_<F>(0.f);
-      }
+      if (RESET && (rs >> i & 1)) a[i] = all_<F>(0.f);
+    }
+    if (n < kSteps) {  // behind the end: the state passes
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i)
+        if (i >= n) {
+          a[i] = all_<F>(1.f);
+          b[i] = all_<F>(0.f);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      if (RESET && (rs >> i & 1)) H = all_<F>(0.f);
       A = mul_(A, a[i]);
       H = fma_(a[i], H, b[i]);
     }
     F entering;
-    F hv = carry_in<F, CLUSTER, false>(maps, (int)(round & 1), A, H, S, entering);
+    F hv = carry_in<F, CLUSTER, false, RESET>(maps, (int)(round & 1), A, H, S, entering);
     if (p.on) {
       if (ckpt && w == 0 && tile < tiles)
         Elem<float, V>::store(ckpt + (p.b * tiles + tile) * C + p.c, entering);
+      T* hp = h + (p.b * L + t0) * C + p.c;
+      auto walk = [&](auto full) {
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        if (RESET && (rs >> i & 1)) hv = all_<F>(0.f);
-        hv = fma_(a[i], hv, b[i]);
-        if (i < n) EX::store(h + (t0 + i) * C, hv);
-      }
+        for (int i = 0; i < kSteps; ++i, hp += C) {
+          if (RESET && (rs >> i & 1)) hv = all_<F>(0.f);
+          hv = fma_(a[i], hv, b[i]);
+          if (full || i < n) EX::store(hp, hv);
+        }
+      };
+      if (n == kSteps) walk(std::true_type{});
+      else walk(std::false_type{});
       // the warp that has the last step
       if (hT && n > 0 && t0 + n == L) Elem<float, V>::store(hT + p.b * C + p.c, hv);
     }
@@ -363,7 +399,28 @@ glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
 template <typename T, typename G, int V> struct BwdRing {
   FwdRing<T, G, V> in;
   uint8_t d[kStages][kWarps][kSteps][32 * Elem<T, V>::kBytes];
+  // lo_b of the round between its first and last walk: in registers it would spill
+  typename Lane<V>::F lo_b[kWarps][kSteps][32];
 };
+
+// Of a logit z: the smaller of sigmoid(z) and 1 - sigmoid(z), with z's sign; from it both follow
+// without cancellation.
+template <typename F> __device__ __forceinline__ F sigmoid_lower(F z) {
+  const F t = map_([](float v) { return ex2(-fabsf(v) * kLog2e); }, z);
+  const F r = map_(rcp, add_(t, all_<F>(1.f)));
+  return map_([](float l, float v) { return copysignf(l, v); }, mul_(t, r), z);
+}
+template <typename F> __device__ __forceinline__ F sigmoid_of(F lo) {
+  return map_([](float l) { return signbit(l) ? -l : 1.f - l; }, lo);
+}
+template <typename F> __device__ __forceinline__ F one_minus_sigmoid_of(F lo) {
+  return map_([](float l) { return signbit(l) ? 1.f + l : l; }, lo);
+}
+
+// Makes the compiler forget what it computed from v: recomputing u, a^2, ... in the last walk is
+// cheaper than keeping them for all steps (they spilled).
+__device__ __forceinline__ void forget(float& v) { asm volatile("" : "+f"(v)); }
+__device__ __forceinline__ void forget(float2& v) { asm volatile("" : "+f"(v.x), "+f"(v.y)); }
 
 template <typename T, typename G, int V, bool LOGITS, bool RESET, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -372,7 +429,7 @@ glr_bwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
                const float* __restrict__ ckpt, const T* __restrict__ dh,
                const float* __restrict__ dhT, T* __restrict__ dx, G* __restrict__ dg,
                G* __restrict__ dbeta, float* __restrict__ dh0, float* __restrict__ ddecay_part,
-               int64_t L, int64_t C, Strides st, float scale) {
+               int64_t L, int64_t C, Strides st, float scale, bool wide) {
   using F = typename Lane<V>::F;
   using EX = Elem<T, V>;
   using EG = Elem<G, V>;
@@ -383,15 +440,10 @@ glr_bwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
   const Place p = place<V, CLUSTER>(C);
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t tiles = (L + kTile - 1) / kTile, rounds = (tiles + p.size - 1) / p.size;
-  if (p.on) {
-    x += p.b * st.xb + p.c;
-    g += p.b * st.gb + p.c;
-    beta += p.b * st.bb + p.c;
-    dh += p.b * L * C + p.c;
-    dx += p.b * L * C + p.c;
-    dg += p.b * L * C + p.c;
-    dbeta += p.b * L * C + p.c;
-  }
+  x += p.b * st.xb + p.c0;
+  g += p.b * st.gb + p.c0;
+  beta += p.b * st.bb + p.c0;
+  dh += p.b * L * C + p.c0;
   if (RESET) reset += p.b * L;
   F rate = all_<F>(0.f), sum = all_<F>(0.f);
   F R = all_<F>(0.f);  // a_t D_t of the step behind the round
@@ -400,19 +452,15 @@ glr_bwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
       rate = map_([&](float d) { return -scale * softplus(d); }, Elem<float, V>::load(decay + p.c));
     if (dhT) R = Elem<float, V>::load(dhT + p.b * C + p.c);
   }
+  auto rows_of = [&](int64_t t0) { return t0 < L ? (int)(L - t0 < kSteps ? L - t0 : kSteps) : 0; };
   auto fetch = [&](int64_t k) {  // k-th round from the end
     const int64_t t0 = ((rounds - 1 - k) * p.size + p.rank) * kTile + w * kSteps;
-    const int s = (int)(k % kStages);
-    if (p.on && k < rounds) {
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        if (t0 + i < L) {
-          EX::copy(&ring.in.x[s][w][i][lane * EX::kBytes], x + (t0 + i) * st.xl);
-          EG::copy(&ring.in.g[s][w][i][lane * EG::kBytes], g + (t0 + i) * st.gl);
-          EG::copy(&ring.in.b[s][w][i][lane * EG::kBytes], beta + (t0 + i) * st.bl);
-          EX::copy(&ring.d[s][w][i][lane * EX::kBytes], dh + (t0 + i) * C);
-        }
-      }
+    const int s = (int)(k % kStages), n = k < rounds ? rows_of(t0) : 0;
+    if (n > 0) {
+      copy_rows<T, V>(ring.in.x[s][w], x + t0 * st.xl, st.xl, C - p.c0, n, wide);
+      copy_rows<G, V>(ring.in.g[s][w], g + t0 * st.gl, st.gl, C - p.c0, n, wide);
+      copy_rows<G, V>(ring.in.b[s][w], beta + t0 * st.bl, st.bl, C - p.c0, n, wide);
+      copy_rows<T, V>(ring.d[s][w], dh + t0 * C, C, C - p.c0, n, wide);
     }
     copy_commit();
   };
@@ -420,108 +468,125 @@ glr_bwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
   for (int k = 0; k < kStages - 1; ++k) fetch(k);
   for (int64_t k = 0; k < rounds; ++k) {
     const int64_t tile = (rounds - 1 - k) * p.size + p.rank, t0 = tile * kTile + w * kSteps;
-    const int n = t0 < L ? (int)(L - t0 < kSteps ? L - t0 : kSteps) : 0;
-    const int s = (int)(k % kStages);
+    const int n = rows_of(t0), s = (int)(k % kStages);
     F first = all_<F>(0.f);  // the state in front of the tile
     if (p.on && tile < tiles) first = Elem<float, V>::load(ckpt + (p.b * tiles + tile) * C + p.c);
     fetch(k + kStages - 1);
     const uint32_t rs = RESET ? reset_bits(reset, t0, L) : 0;
     copy_wait<kStages - 1>();
-    // The gates of the steps.  lo_g, lo_b: the smaller of sigmoid and 1 - sigmoid, with the
-    // logit's sign, from which both follow without cancellation (values: beta and x).
-    F a[kSteps], m[kSteps], lo_g[kSteps], lo_b[kSteps], xv[kSteps], dv[kSteps];
+    if (n < kSteps) {  // behind the end nothing comes in
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i)
+        if (i >= n) {
+          EX::zero(&ring.in.x[s][w][i][lane * EX::kBytes]);
+          EX::zero(&ring.d[s][w][i][lane * EX::kBytes]);
+          EG::zero(&ring.in.g[s][w][i][lane * EG::kBytes]);
+          EG::zero(&ring.in.b[s][w][i][lane * EG::kBytes]);
+        }
+    }
+    __syncwarp();
+    auto x_of = [&](int i) { return EX::load(&ring.in.x[s][w][i][lane * EX::kBytes]); };
+    auto beta_of = [&](int i) { return EG::load(&ring.in.b[s][w][i][lane * EG::kBytes]); };
+    auto d_of = [&](int i) { return EX::load(&ring.d[s][w][i][lane * EX::kBytes]); };
+    // What the walks need of the gates; x and dh are read again from the ring.
+    F a[kSteps], m[kSteps], lo_g[kSteps];  // values: only a
+    F(&lo_b)[kSteps][32] = ring.lo_b[w];
+    auto b_of = [&](int i) {
+      if (LOGITS) return mul_(mul_(m[i], sigmoid_of(lo_b[i][lane])), x_of(i));
+      return mul_(beta_of(i), x_of(i));
+    };
     F A = all_<F>(1.f), H = all_<F>(0.f), Q = all_<F>(0.f);
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-      xv[i] = EX::load(&ring.in.x[s][w][i][lane * EX::kBytes]);
-      dv[i] = EX::load(&ring.d[s][w][i][lane * EX::kBytes]);
       const F gv = EG::load(&ring.in.g[s][w][i][lane * EG::kBytes]);
-      const F bv = EG::load(&ring.in.b[s][w][i][lane * EG::kBytes]);
       F b;
       if (LOGITS) {
-        auto lower = [](float z) {
-          const float t = ex2(-fabsf(z) * kLog2e);
-          return copysignf(t * rcp(1.f + t), z);
-        };
-        // sigmoid from the smaller part
-        auto sig = [](float l) { return signbit(l) ? -l : 1.f - l; };
-        lo_g[i] = map_(lower, gv);
-        lo_b[i] = map_(lower, bv);
-        const F u = mul_(rate, map_(sig, lo_g[i]));
-        a[i] = map_([](float z) { return ex2(z * kLog2e); }, u);
+        lo_g[i] = sigmoid_lower(gv);
+        const F lb = sigmoid_lower(beta_of(i));
+        lo_b[i][lane] = lb;
+        const F u = mul_(rate, sigmoid_of(lo_g[i]));
+        a[i] = map_(ex2, mul_(u, all_<F>(kLog2e)));
         m[i] = map_(sqrt_, one_minus_exp(mul_(u, all_<F>(-2.f)), mul_(a[i], a[i])));
         if (RESET && (rs >> i & 1)) m[i] = all_<F>(1.f);
-        b = mul_(mul_(m[i], map_(sig, lo_b[i])), xv[i]);
+        b = mul_(mul_(m[i], sigmoid_of(lb)), x_of(i));
       } else {
         a[i] = gv;
-        lo_b[i] = bv;
-        b = mul_(bv, xv[i]);
+        b = mul_(beta_of(i), x_of(i));
       }
       if (RESET && (rs >> i & 1)) {
         a[i] = all_<F>(0.f);
         H = all_<F>(0.f);
       }
-      if (i >= n) {
-        a[i] = all_<F>(1.f);
-        xv[i] = b = dv[i] = all_<F>(0.f);
-      }
+      if (i >= n) a[i] = all_<F>(1.f);  // behind the end: the state passes
       A = mul_(A, a[i]);
       H = fma_(a[i], H, b);
     }
 #pragma unroll
     for (int i = kSteps - 1; i >= 0; --i) {  // Q: D of step i, without what enters
-      if (i + 1 < kSteps) Q = RESET && (rs >> (i + 1) & 1) ? dv[i] : fma_(a[i + 1], Q, dv[i]);
-      else Q = dv[i];
+      if (i + 1 < kSteps) Q = RESET && (rs >> (i + 1) & 1) ? d_of(i) : fma_(a[i + 1], Q, d_of(i));
+      else Q = d_of(i);
     }
     Q = RESET && (rs & 1) ? all_<F>(0.f) : mul_(a[0], Q);
     F unused;
-    F hv = carry_in<F, false, false>(fwd_maps, (int)(k & 1), A, H, first, unused);
-    F d = carry_in<F, CLUSTER, true>(maps, (int)(k & 1), A, Q, R, unused);
+    F hv = carry_in<F, false, false, RESET>(fwd_maps, (int)(k & 1), A, H, first, unused);
+    F d = carry_in<F, CLUSTER, true, RESET>(maps, (int)(k & 1), A, Q, R, unused);
     if (p.on) {
-    F before[kSteps];
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      before[i] = hv;
-      F b;
-      if (LOGITS)
-        b = mul_(mul_(m[i], map_([](float l) { return signbit(l) ? -l : 1.f - l; }, lo_b[i])), xv[i]);
-      else
-        b = mul_(lo_b[i], xv[i]);
-      if (RESET && (rs >> i & 1)) hv = all_<F>(0.f);
-      hv = fma_(a[i], hv, b);
-    }
+      for (int i = 0; i < kSteps; ++i) {
+        forget(a[i]);
+        if (LOGITS) {
+          forget(lo_g[i]);
+          forget(m[i]);
+        }
+      }
+      F before[kSteps];
 #pragma unroll
-    for (int i = kSteps - 1; i >= 0; --i) {
-      const bool zero = RESET && (rs >> i & 1);
-      if (i + 1 == kSteps) d = add_(d, dv[i]);
-      else d = RESET && (rs >> (i + 1) & 1) ? dv[i] : fma_(a[i + 1], d, dv[i]);
-      F ox, og, ob;
-      if (LOGITS) {
-        auto small = [](float l) { return signbit(l) ? -l : 1.f - l; };
-        auto large = [](float l) { return signbit(l) ? 1.f + l : l; };  // 1 - sigmoid
-        const F u = mul_(rate, map_(small, lo_g[i]));
-        const F mi = mul_(m[i], map_(small, lo_b[i])), b = mul_(mi, xv[i]);
-        // a^2 / (1 - a^2); a == 1 leaves the limit 0 of (that * u * b)
-        const F q = map_([](float m_, float a_) { return m_ > 1e-18f ? a_ * a_ * rcp(m_ * m_) : 0.f; },
-                         m[i], a[i]);
-        F du = mul_(d, fma_(a[i], before[i], mul_(mul_(q, b), all_<F>(-1.f))));
-        if (zero) du = all_<F>(0.f);
-        if (i < n) sum = fma_(du, u, sum);
-        og = mul_(mul_(du, u), map_(large, lo_g[i]));
-        ox = mul_(d, mi);
-        ob = mul_(mul_(d, b), map_(large, lo_b[i]));
-      } else {
-        ox = mul_(d, lo_b[i]);
-        ob = mul_(d, xv[i]);
-        og = zero ? all_<F>(0.f) : mul_(d, before[i]);
+      for (int i = 0; i < kSteps; ++i) {
+        before[i] = hv;
+        if (RESET && (rs >> i & 1)) hv = all_<F>(0.f);
+        hv = fma_(a[i], hv, b_of(i));
       }
-      if (i < n) {
-        const int64_t o = (t0 + i) * C;
-        EX::store(dx + o, ox);
-        EG::store(dg + o, og);
-        EG::store(dbeta + o, ob);
-      }
-    }
+#pragma unroll
+      for (int i = 0; LOGITS && i < kSteps; ++i) forget(m[i]);
+      asm volatile("" ::: "memory");
+      int64_t o = (p.b * L + t0 + kSteps - 1) * C + p.c;
+      auto walk = [&](auto full) {
+#pragma unroll
+        for (int i = kSteps - 1; i >= 0; --i, o -= C) {
+          const bool zero = RESET && (rs >> i & 1);
+          const F xv = x_of(i);
+          if (i + 1 == kSteps) d = add_(d, d_of(i));
+          else d = RESET && (rs >> (i + 1) & 1) ? d_of(i) : fma_(a[i + 1], d, d_of(i));
+          F ox, og, ob;
+          if (LOGITS) {
+            const F u = mul_(rate, sigmoid_of(lo_g[i]));
+            const F lb = lo_b[i][lane];
+            const F mi = mul_(m[i], sigmoid_of(lb)), b = mul_(mi, xv);
+            // a^2 / (1 - a^2); a == 1 leaves the limit 0 of (that * u * b)
+            const F q = map_(
+                [](float m_, float v, float a2) { return m_ > 1e-18f ? a2 * rcp(v) : 0.f; }, m[i],
+                mul_(m[i], m[i]), mul_(a[i], a[i]));
+            F du = mul_(d, fma_(a[i], before[i], mul_(mul_(q, b), all_<F>(-1.f))));
+            if (zero) du = all_<F>(0.f);
+            if (full || i < n) sum = fma_(du, u, sum);
+            og = mul_(mul_(du, u), one_minus_sigmoid_of(lo_g[i]));
+            ox = mul_(d, mi);
+            ob = mul_(mul_(d, b), one_minus_sigmoid_of(lb));
+          } else {
+            ox = mul_(d, beta_of(i));
+            ob = mul_(d, xv);
+            og = zero ? all_<F>(0.f) : mul_(d, before[i]);
+          }
+          if (full || i < n) {
+            EX::store(dx + o, ox);
+            EG::store(dg + o, og);
+            EG::store(dbeta + o, ob);
+          }
+        }
+      };
+      if (n == kSteps) walk(std::true_type{});
+      else walk(std::false_type{});
     }
     __syncwarp();
   }
@@ -632,14 +697,27 @@ bool multiple(const void* p, int64_t bytes) {
   return reinterpret_cast<uintptr_t>(p) % bytes == 0;
 }
 
-// Two channels a lane: pairs have to start at a multiple of their size everywhere.
+// Two channels a lane (packed arithmetic, 128-byte rows of a warp), for 16-bit gates and where
+// pairs start at a multiple of their size everywhere.  fp32 rows of a warp are 128 bytes as they
+// are, and pairs of them would leave room for one CTA on an SM instead of two.
 bool pairs_ok(const void* const* xs, int nx, const void* const* gs, int ng, const void* const* fs,
               int nf, const int64_t* strides, int64_t C, int xbytes, int gbytes) {
-  bool ok = C % 2 == 0;
+  bool ok = gbytes == 2 && C % 2 == 0;
   for (int i = 0; i < nx; ++i) ok = ok && multiple(xs[i], 2 * xbytes);
   for (int i = 0; i < ng; ++i) ok = ok && multiple(gs[i], 2 * gbytes);
   for (int i = 0; i < nf; ++i) ok = ok && multiple(fs[i], 8);
   for (int i = 0; i < 6; ++i) ok = ok && strides[i] % 2 == 0;
+  return ok;
+}
+
+// 16-byte copies: rows have to start at, and be, multiples of 16 bytes.
+bool wide_ok(const void* const* xs, int nx, const void* const* gs, int ng, const int64_t* strides,
+             int64_t C, int xbytes, int gbytes) {
+  const int px = 16 / xbytes, pg = 16 / gbytes, least = px < pg ? pg : px;
+  bool ok = C % least == 0;
+  for (int i = 0; i < nx; ++i) ok = ok && multiple(xs[i], 16);
+  for (int i = 0; i < ng; ++i) ok = ok && multiple(gs[i], 16);
+  for (int i = 0; i < 6; ++i) ok = ok && strides[i] % least == 0;
   return ok;
 }
 
@@ -702,13 +780,14 @@ extern "C" int fo_glr_fwd(const void* x, const void* g, const void* beta, const 
     using G = decltype(gt);
     const void *xs[] = {x, h}, *gs[] = {g, beta}, *fs[] = {decay, h0, hT, ckpt};
     const bool two = pairs_ok(xs, 2, gs, 2, fs, 4, q, C, sizeof(T), sizeof(G));
+    const bool wide = wide_ok(xs, 1, gs, 2, q, C, sizeof(T), sizeof(G));
     const int64_t ctas = B * slabs_of(C, two ? 2 : 1);
     const int cl = cluster_for(ctas, L, 2 * num_sms());
     return with_flags(two, decay, reset, cl > 1, [&](auto tw, auto lo, auto rs, auto c) {
-      constexpr int V = tw ? 2 : 1;
+      constexpr int V = tw && sizeof(G) == 2 ? 2 : 1;
       return launch("glr_fwd_kernel", glr_fwd_kernel<T, G, V, lo, rs, c>, ctas, cl,
                     (int)sizeof(FwdRing<T, G, V>), as_stream(stream), (const T*)x, (const G*)g,
-                    (const G*)beta, decay, h0, reset, (T*)h, hT, ckpt, L, C, s, scale);
+                    (const G*)beta, decay, h0, reset, (T*)h, hT, ckpt, L, C, s, scale, wide);
     });
   });
 }
@@ -775,14 +854,15 @@ extern "C" int fo_glr_bwd(const void* x, const void* g, const void* beta, const 
     using G = decltype(gt);
     const void *xs[] = {x, dh, dx}, *gs[] = {g, beta, dg, dbeta}, *fs[] = {decay, ckpt, dhT, dh0};
     const bool two = pairs_ok(xs, 3, gs, 4, fs, 4, sq, C, sizeof(T), sizeof(G));
+    const bool wide = wide_ok(xs, 2, gs, 2, sq, C, sizeof(T), sizeof(G));
     const int64_t ctas = B * slabs_of(C, two ? 2 : 1);
     const int cl = cluster_for(ctas, L, 2 * num_sms());
     int rc = with_flags(two, decay, reset, cl > 1, [&](auto tw, auto lo, auto rs, auto c) {
-      constexpr int V = tw ? 2 : 1;
+      constexpr int V = tw && sizeof(G) == 2 ? 2 : 1;
       return launch("glr_bwd_kernel", glr_bwd_kernel<T, G, V, lo, rs, c>, ctas, cl,
                     (int)sizeof(BwdRing<T, G, V>), q, (const T*)x, (const G*)g, (const G*)beta,
                     decay, reset, ckpt, (const T*)dh, dhT, (T*)dx, (G*)dg, (G*)dbeta, dh0, part,
-                    L, C, s, scale);
+                    L, C, s, scale, wide);
     });
     if (rc || !ddecay) return rc;
     glr_ddecay_kernel<<<(unsigned)((C + 127) / 128), 128, 0, q>>>(part, B * cl, decay, ddecay, C);
