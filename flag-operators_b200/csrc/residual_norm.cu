@@ -14,6 +14,16 @@
 // the rounding of the stored r'.  mean(k y) needs D, which needs mean(e r'); writing
 //   sum k y = sum q y (dr' + inv2 e) - c2 sum q y r',  q = s act w_post, c2 = inv2^3 mean(e r')
 // gets all three sums of a row from one pass and one block reduction.
+//
+// Both are bound by memory.  Where rows are 16-byte aligned and fit, TPR threads own a row, VPT
+// 16-byte vectors each, and CTAs walk over the rows: every input is read once, by cp.async into a
+// ring of two rows in shared memory (the next row is on its way while this one is reduced and
+// written), and a thread only ever reads the slots that it filled, so the ring needs no barrier.
+// The backward keeps its threads' column sums in registers over all rows of the CTA, writes them
+// as one partial row a CTA, and a column kernel adds those up in their order.  Other widths take
+// the generic kernels: several passes over the row, through L1 and L2.
+#include <type_traits>
+
 #include "gates.cuh"
 
 namespace fo {
@@ -59,7 +69,327 @@ __device__ __forceinline__ void act_grad(int act, float z, float& a, float& da) 
   da = act == FO_ACT_SILU ? s * fmaf(z, c, 1.f) : s * c;
 }
 
-// Any width and alignment: a CTA per row, three passes over it (the later ones from L1 / L2).
+// ---------------------------------------------------------------------------
+// Rows in a shared-memory ring
+// ---------------------------------------------------------------------------
+template <int TPR> struct Shape {
+  static constexpr int kThreads = TPR > 256 ? TPR : TPR > 32 ? TPR : 256;
+  static constexpr int kRows = kThreads / TPR;  // rows side by side in a CTA
+};
+
+// Streams [S] of rows in two stages; slot(s, k, i): vector i of stream k in stage s, of this thread.
+template <int S, int VPT, int THREADS> struct Ring {
+  uint4 v[2][S][VPT][THREADS];
+  __device__ __forceinline__ uint4& slot(int s, int k, int i) { return v[s][k][i][threadIdx.x]; }
+  __device__ __forceinline__ void fetch(int s, int k, int i, const void* p) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                     (uint32_t)__cvta_generic_to_shared(&slot(s, k, i))),
+                 "l"(p)
+                 : "memory");
+  }
+};
+__device__ __forceinline__ void ring_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void ring_wait_one() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+
+// Sums of K values over the TPR threads of a row, in every one of them.  `red`: [K][warps], not
+// used by the reduction before this one.
+template <int TPR, int K>
+__device__ __forceinline__ void row_sum(float (&v)[K], float (*red)[32]) {
+#pragma unroll
+  for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  if constexpr (TPR > 32) {
+    constexpr int kWarps = TPR / 32;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    if (lane == 0)
+#pragma unroll
+      for (int k = 0; k < K; ++k) red[k][w] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = red[k][lane % kWarps];
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1)
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  }
+}
+
+// f *= the weights' vector v (f *= number where there is none)
+template <typename W, int E>
+__device__ __forceinline__ void times(float (&f)[E], const W* w, int v, float number) {
+  if (w) {
+    float t[E];
+    constexpr int kPer = Vec16<W>::E;  // fp32 weights of 16-bit rows: two loads a vector
+#pragma unroll
+    for (int e = 0; e < E; e += kPer) unpack16<W>(ld_global_nc_v4(w + (int64_t)v * E + e), t + e);
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] *= t[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] *= number;
+  }
+}
+
+template <typename T, typename W, int TPR, int VPT>
+__global__ void __launch_bounds__(Shape<TPR>::kThreads, 1024 / Shape<TPR>::kThreads)
+rrn_fwd_kernel(Fwd a) {
+  using S = Shape<TPR>;
+  constexpr int E = Vec16<T>::E;
+  extern __shared__ __align__(16) uint8_t smem[];
+  auto& ring = *reinterpret_cast<Ring<3, VPT, S::kThreads>*>(smem);
+  __shared__ float red[4][32];
+  const W *w = (const W*)a.w, *wp = (const W*)a.wp, *sv = (const W*)a.sv;
+  const int nvec = (int)(a.N / E), v0 = threadIdx.x % TPR;
+  const float n = (float)a.N;
+  const int64_t step = (int64_t)gridDim.x * S::kRows, mine = threadIdx.x / TPR;
+  auto fetch = [&](int64_t base, int s) {
+    const int64_t row = base + mine;
+    if (row < a.M) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int v = v0 + i * TPR;
+        if (v < nvec) {
+          ring.fetch(s, 0, i, (const T*)a.y + row * a.y_ld + v * E);
+          ring.fetch(s, 1, i, (const T*)a.r + row * a.r_ld + v * E);
+          if (a.gate) ring.fetch(s, 2, i, (const T*)a.gate + row * a.g_ld + v * E);
+        }
+      }
+    }
+    ring_commit();
+  };
+  int64_t base = (int64_t)blockIdx.x * S::kRows;
+  fetch(base, 0);
+  for (int it = 0; base < a.M; base += step, ++it) {
+    const int s = it & 1;
+    fetch(base + step, s ^ 1);
+    ring_wait_one();
+    const int64_t row = base + mine;
+    const bool on = row < a.M;
+    float inv1 = 1.f;
+    if (wp) {
+      float ss[1] = {0.f};
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+        if (on && v0 + i * TPR < nvec) {
+          float f[E];
+          unpack16<T>(ring.slot(s, 0, i), f);
+#pragma unroll
+          for (int e = 0; e < E; ++e) ss[0] = fmaf(f[e], f[e], ss[0]);
+        }
+      row_sum<TPR>(ss, red + s);
+      inv1 = 1.f / sqrtf(ss[0] / n + a.eps);
+    }
+    float r2[VPT][E], ss[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = v0 + i * TPR;
+      if (on && v < nvec) {
+        float u[E];
+        unpack16<T>(ring.slot(s, 0, i), u);
+#pragma unroll
+        for (int e = 0; e < E; ++e) u[e] *= inv1;
+        if (wp) times<W>(u, wp, v, 1.f);
+        if (a.gate) {
+          float z[E];
+          unpack16<T>(ring.slot(s, 2, i), z);
+#pragma unroll
+          for (int e = 0; e < E; ++e) u[e] *= act_of(a.act, z[e]);
+        }
+        times<W>(u, sv, v, a.s);
+        float r[E];
+        unpack16<T>(ring.slot(s, 1, i), r);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          r2[i][e] = r[e] + u[e];
+          ss[0] = fmaf(r2[i][e], r2[i][e], ss[0]);
+        }
+      }
+    }
+    row_sum<TPR>(ss, red + 2 + s);
+    const float inv2 = 1.f / sqrtf(ss[0] / n + a.eps);
+    if (on && v0 == 0) {
+      if (a.inv1) a.inv1[row] = inv1;
+      if (a.inv2) a.inv2[row] = inv2;
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = v0 + i * TPR;
+      if (on && v < nvec) {
+        st_global_stream_v4((T*)a.res + row * a.N + v * E, pack16<T>(r2[i]));
+#pragma unroll
+        for (int e = 0; e < E; ++e) r2[i][e] *= inv2;
+        times<W>(r2[i], w, v, 1.f);
+        st_global_stream_v4((T*)a.out + row * a.N + v * E, pack16<T>(r2[i]));
+      }
+    }
+  }
+}
+
+template <typename T, typename W, int TPR, int VPT>
+__global__ void __launch_bounds__(Shape<TPR>::kThreads, 512 / Shape<TPR>::kThreads)
+rrn_bwd_kernel(Bwd a) {
+  using S = Shape<TPR>;
+  constexpr int E = Vec16<T>::E;
+  extern __shared__ __align__(16) uint8_t smem[];
+  auto& ring = *reinterpret_cast<Ring<5, VPT, S::kThreads>*>(smem);
+  __shared__ float red[6][32];
+  const W *w = (const W*)a.w, *wp = (const W*)a.wp, *sv = (const W*)a.sv;
+  const int nvec = (int)(a.N / E), v0 = threadIdx.x % TPR;
+  const int64_t step = (int64_t)gridDim.x * S::kRows, mine = threadIdx.x / TPR;
+  auto fetch = [&](int64_t base, int s) {
+    const int64_t row = base + mine;
+    if (row < a.M) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int v = v0 + i * TPR;
+        if (v < nvec) {
+          ring.fetch(s, 0, i, (const T*)a.y + row * a.y_ld + v * E);
+          ring.fetch(s, 1, i, (const T*)a.r + row * a.r_ld + v * E);
+          if (a.gate) ring.fetch(s, 2, i, (const T*)a.gate + row * a.g_ld + v * E);
+          if (a.dout) ring.fetch(s, 3, i, (const T*)a.dout + row * a.N + v * E);
+          if (a.dres) ring.fetch(s, 4, i, (const T*)a.dres + row * a.N + v * E);
+        }
+      }
+    }
+    ring_commit();
+  };
+  // Of a vector: y, p / inv1 = y w_post, act and act', s, r', d, e, dr'
+  struct Part {
+    float y[E], q[E], av[E], da[E], sj[E], r2[E], d[E], e[E], dr[E];
+  };
+  auto load = [&](int s, int i, int v, float inv1, Part& p) {
+    unpack16<T>(ring.slot(s, 0, i), p.y);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      p.q[e] = p.y[e];
+      p.sj[e] = 1.f;
+      p.av[e] = 1.f;
+      p.da[e] = 0.f;
+      p.d[e] = p.dr[e] = 0.f;
+    }
+    if (wp) times<W>(p.q, wp, v, 1.f);
+    times<W>(p.sj, sv, v, a.s);
+    if (a.gate) {
+      float z[E];
+      unpack16<T>(ring.slot(s, 2, i), z);
+#pragma unroll
+      for (int e = 0; e < E; ++e) act_grad(a.act, z[e], p.av[e], p.da[e]);
+    }
+    unpack16<T>(ring.slot(s, 1, i), p.r2);
+#pragma unroll
+    for (int e = 0; e < E; ++e) p.r2[e] = fmaf(p.sj[e] * p.av[e], inv1 * p.q[e], p.r2[e]);
+    if (a.dout) unpack16<T>(ring.slot(s, 3, i), p.d);
+#pragma unroll
+    for (int e = 0; e < E; ++e) p.e[e] = p.d[e];
+    times<W>(p.e, w, v, 1.f);
+    if (a.dres) unpack16<T>(ring.slot(s, 4, i), p.dr);
+  };
+  float dw[VPT][E], ds[VPT][E], dwp[VPT][E];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)
+#pragma unroll
+    for (int e = 0; e < E; ++e) dw[i][e] = ds[i][e] = dwp[i][e] = 0.f;
+  int64_t base = (int64_t)blockIdx.x * S::kRows;
+  fetch(base, 0);
+  for (int it = 0; base < a.M; base += step, ++it) {
+    const int s = it & 1;
+    fetch(base + step, s ^ 1);
+    const int64_t row = base + mine;
+    const bool on = row < a.M;
+    const float inv1 = wp && on ? a.inv1[row] : 1.f, inv2 = on ? a.inv2[row] : 1.f;
+    ring_wait_one();
+    float sum[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = v0 + i * TPR;
+      if (on && v < nvec) {
+        Part p;
+        load(s, i, v, inv1, p);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float qy = p.sj[e] * p.av[e] * p.q[e];
+          sum[0] = fmaf(p.e[e], p.r2[e], sum[0]);
+          sum[1] = fmaf(qy, fmaf(inv2, p.e[e], p.dr[e]), sum[1]);
+          sum[2] = fmaf(qy, p.r2[e], sum[2]);
+        }
+      }
+    }
+    row_sum<TPR>(sum, red + 3 * s);
+    const float c2 = inv2 * inv2 * inv2 * sum[0] / (float)a.N;
+    const float c1 = wp ? inv1 * inv1 * inv1 * fmaf(-c2, sum[2], sum[1]) / (float)a.N : 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = v0 + i * TPR;
+      if (on && v < nvec) {
+        Part p;
+        load(s, i, v, inv1, p);
+        float dr[E], dy[E], dg[E], k[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float D = fmaf(inv2, p.e[e], fmaf(-c2, p.r2[e], p.dr[e]));
+          const float pe = p.q[e] * inv1, sD = p.sj[e] * D;
+          dr[e] = D;
+          dg[e] = sD * pe * p.da[e];
+          k[e] = sD * p.av[e];
+          dw[i][e] = fmaf(p.d[e] * p.r2[e], inv2, dw[i][e]);
+          ds[i][e] = fmaf(D, p.av[e] * pe, ds[i][e]);
+          dwp[i][e] = fmaf(k[e], p.y[e] * inv1, dwp[i][e]);
+        }
+        if (wp) times<W>(k, wp, v, 1.f);
+#pragma unroll
+        for (int e = 0; e < E; ++e) dy[e] = fmaf(inv1, k[e], -c1 * p.y[e]);
+        st_global_stream_v4((T*)a.dr + row * a.N + v * E, pack16<T>(dr));
+        st_global_stream_v4((T*)a.dy + row * a.N + v * E, pack16<T>(dy));
+        if (a.gate) st_global_stream_v4((T*)a.dgate + row * a.N + v * E, pack16<T>(dg));
+      }
+    }
+  }
+  // part[3][gridDim.x][N]; rows side by side in the CTA are added up first
+  const int64_t stride = (int64_t)gridDim.x * a.N;
+  float* part = a.part + (int64_t)blockIdx.x * a.N;
+  if constexpr (S::kRows == 1) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = v0 + i * TPR;
+      if (v < nvec)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          part[v * E + e] = dw[i][e];
+          part[stride + v * E + e] = ds[i][e];
+          part[2 * stride + v * E + e] = dwp[i][e];
+        }
+    }
+  } else {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    float* sums = reinterpret_cast<float*>(smem);  // [rows][3][N], over the ring
+    __syncthreads();
+    const int N = (int)a.N;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = v0 + i * TPR;
+      if (v < nvec)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          float* to = sums + mine * 3 * N + v * E + e;
+          to[0] = dw[i][e];
+          to[N] = ds[i][e];
+          to[2 * N] = dwp[i][e];
+        }
+    }
+    __syncthreads();
+    for (int j = threadIdx.x; j < 3 * N; j += S::kThreads) {
+      float t = 0.f;
+      for (int r = 0; r < S::kRows; ++r) t += sums[r * 3 * N + j];
+      part[j / N * stride + j % N] = t;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Any width and alignment
+// ---------------------------------------------------------------------------
+// A CTA per row, three passes over it (the later ones from L1 / L2).
 template <typename T, typename W>
 __global__ void __launch_bounds__(256) rrn_fwd_generic_kernel(Fwd a) {
   __shared__ float red[32];
@@ -182,16 +512,30 @@ __global__ void __launch_bounds__(256) rrn_cols_kernel(Bwd a) {
   part[2 * step] = dwp;
 }
 
-// dw, ds, dw_post from the partial rows, added in their order.
+// dw, ds, dw_post from the G partial rows.  A CTA owns 32 columns; warp q adds the rows q, q + 16,
+// ..., then warp 0 the 16 warps' sums: an order that does not depend on scheduling.
+constexpr int kReduceWarps = 16;
 template <typename W>
-__global__ void __launch_bounds__(128) rrn_reduce_kernel(Bwd a, int G) {
-  const int64_t j = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+__global__ void __launch_bounds__(32 * kReduceWarps) rrn_reduce_kernel(Bwd a, int G) {
+  __shared__ float acc[kReduceWarps][33];
+  const int lane = threadIdx.x & 31, q = threadIdx.x >> 5;
+  const int64_t j = (int64_t)blockIdx.x * 32 + lane;
   W* to = (W*)(blockIdx.y == 0 ? a.dw : blockIdx.y == 1 ? a.ds : a.dwp);
-  if (j >= a.N || !to) return;
-  const float* p = a.part + blockIdx.y * (int64_t)G * a.N + j;
+  if (!to) return;
   float t = 0.f;
-  for (int k = 0; k < G; ++k) t += p[(int64_t)k * a.N];
-  to[j] = from_f<W>(t);
+  if (j < a.N) {
+    const float* p = a.part + blockIdx.y * (int64_t)G * a.N + j;
+#pragma unroll 4
+    for (int k = q; k < G; k += kReduceWarps) t += p[(int64_t)k * a.N];
+  }
+  acc[q][lane] = t;
+  __syncthreads();
+  if (q == 0 && j < a.N) {
+    t = 0.f;
+#pragma unroll
+    for (int k = 0; k < kReduceWarps; ++k) t += acc[k][lane];
+    to[j] = from_f<W>(t);
+  }
 }
 
 unsigned row_grid(int64_t M) {
@@ -199,22 +543,108 @@ unsigned row_grid(int64_t M) {
   return (unsigned)(g < M ? g : M);
 }
 
-int chunks_of(int64_t M) { return (int)(M < kChunks ? (M > 0 ? M : 1) : kChunks); }
+// Partial rows of the column sums, at most: the generic kernel's chunks, or the CTAs of the ring
+// kernel (eight an SM for narrow rows, whose CTAs are small, one for wide ones).
+int64_t partial_rows(int64_t M, int64_t N) {
+  const int64_t per = N <= 1024 ? 8 : N <= 2048 ? 4 : N <= 4096 ? 2 : 1;
+  int64_t g = per * num_sms();
+  if (g < kChunks) g = kChunks;
+  return g < M ? g : (M > 0 ? M : 1);
+}
+
+template <typename T, typename W> constexpr int kMostVectors = 1024;
+
+// Calls f(TPR, VPT) with the smallest shape whose threads cover nvec vectors: a warp or less for
+// the narrowest rows (no barrier), else a CTA of up to 512 threads with one or two vectors each.
+template <typename F> int with_shape(int64_t nvec, F&& f) {
+  auto go = [&](auto tpr, auto vpt) { return f(tpr, vpt); };
+  using std::integral_constant;
+  if (nvec <= 8) return go(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+  if (nvec <= 32) return go(integral_constant<int, 32>{}, integral_constant<int, 1>{});
+  if (nvec <= 64) return go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+  if (nvec <= 128) return go(integral_constant<int, 128>{}, integral_constant<int, 1>{});
+  if (nvec <= 256) return go(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+  if (nvec <= 512) return go(integral_constant<int, 512>{}, integral_constant<int, 1>{});
+  return go(integral_constant<int, 512>{}, integral_constant<int, 2>{});
+}
+
+template <typename T, typename W>
+bool ring_ok(int64_t N, const void* const* rows, const int64_t* lds, int n,
+             const void* const* vectors, int nv) {
+  constexpr int E = Vec16<T>::E;
+  bool ok = N % E == 0 && N / E <= kMostVectors<T, W>;
+  for (int i = 0; i < n; ++i) ok = ok && aligned16(rows[i]) && lds[i] % E == 0;
+  for (int i = 0; i < nv; ++i) ok = ok && aligned16(vectors[i]);
+  return ok;
+}
+
+template <typename K, typename A>
+int launch_ring(const char* what, K kernel, int64_t ctas, int threads, int smem, const A& a,
+                cudaStream_t st) {
+  if (smem > 40 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      set_error("%s: %s", what, cudaGetErrorString(e));
+      return FO_ECUDA;
+    }
+  }
+  kernel<<<(unsigned)ctas, threads, smem, st>>>(a);
+  return check_launch(what);
+}
+
+// CTAs of an SM: by threads (with the registers that they are compiled for), and by shared memory.
+int64_t resident(int threads_per_sm, int threads, int smem) {
+  const int64_t a = threads_per_sm / threads, b = 227 * 1024 / (smem + 2048);
+  return a < b ? a : b;
+}
 
 template <typename T, typename W>
 int run_fwd(const Fwd& a, cudaStream_t st) {
+  const void *rows[] = {a.y, a.r, a.gate, a.out, a.res}, *vs[] = {a.w, a.wp, a.sv};
+  const int64_t lds[] = {a.y_ld, a.r_ld, a.g_ld, a.N, a.N};
+  if (ring_ok<T, W>(a.N, rows, lds, 5, vs, 3))
+    return with_shape(a.N / Vec16<T>::E, [&](auto tpr, auto vpt) {
+      using S = Shape<tpr>;
+      constexpr int smem = (int)sizeof(Ring<3, vpt, S::kThreads>);
+      const int64_t most = num_sms() * resident(1024, S::kThreads, smem);
+      const int64_t need = (a.M + S::kRows - 1) / S::kRows;
+      return launch_ring("rrn_fwd_kernel", rrn_fwd_kernel<T, W, tpr, vpt>,
+                         need < most ? need : most, S::kThreads, smem, a, st);
+    });
   rrn_fwd_generic_kernel<T, W><<<row_grid(a.M), 256, 0, st>>>(a);
   return check_launch("rrn_fwd_generic_kernel");
 }
 
 template <typename T, typename W>
 int run_bwd(const Bwd& a, cudaStream_t st) {
-  rrn_bwd_generic_kernel<T, W><<<row_grid(a.M), 256, 0, st>>>(a);
-  if (int rc = check_launch("rrn_bwd_generic_kernel")) return rc;
-  const int G = chunks_of(a.M);
-  rrn_cols_kernel<T, W><<<dim3((unsigned)((a.N + 255) / 256), G), 256, 0, st>>>(a);
-  if (int rc = check_launch("rrn_cols_kernel")) return rc;
-  rrn_reduce_kernel<W><<<dim3((unsigned)((a.N + 127) / 128), 3), 128, 0, st>>>(a, G);
+  const void *rows[] = {a.y, a.r, a.gate, a.dout, a.dres, a.dy, a.dr, a.dgate},
+             *vs[] = {a.w, a.wp, a.sv};
+  const int64_t lds[] = {a.y_ld, a.r_ld, a.g_ld, a.N, a.N, a.N, a.N, a.N};
+  int G = 0;
+  if (ring_ok<T, W>(a.N, rows, lds, 8, vs, 3)) {
+    const int rc = with_shape(a.N / Vec16<T>::E, [&](auto tpr, auto vpt) {
+      using S = Shape<tpr>;
+      constexpr int ring = (int)sizeof(Ring<5, vpt, S::kThreads>);
+      const int sums = S::kRows > 1 ? (int)(S::kRows * 3 * a.N * 4) : 0;
+      const int smem = ring > sums ? ring : sums;
+      int64_t ctas = num_sms() * resident(512, S::kThreads, smem);
+      const int64_t need = (a.M + S::kRows - 1) / S::kRows, most = partial_rows(a.M, a.N);
+      if (ctas > need) ctas = need;
+      if (ctas > most) ctas = most;
+      G = (int)ctas;
+      return launch_ring("rrn_bwd_kernel", rrn_bwd_kernel<T, W, tpr, vpt>, ctas, S::kThreads, smem,
+                         a, st);
+    });
+    if (rc) return rc;
+  } else {
+    rrn_bwd_generic_kernel<T, W><<<row_grid(a.M), 256, 0, st>>>(a);
+    if (int rc = check_launch("rrn_bwd_generic_kernel")) return rc;
+    G = (int)(a.M < kChunks ? a.M : kChunks);
+    rrn_cols_kernel<T, W><<<dim3((unsigned)((a.N + 255) / 256), G), 256, 0, st>>>(a);
+    if (int rc = check_launch("rrn_cols_kernel")) return rc;
+  }
+  rrn_reduce_kernel<W><<<dim3((unsigned)((a.N + 31) / 32), 3), 32 * kReduceWarps, 0, st>>>(a, G);
   return check_launch("rrn_reduce_kernel");
 }
 
@@ -272,7 +702,7 @@ extern "C" int fo_residual_rms_norm_fwd(
 extern "C" int fo_residual_rms_norm_bwd_workspace_bytes(int64_t M, int64_t N, int64_t* bytes) {
   clear_error();
   FO_CHECK_ARG(bytes && M >= 0 && N > 0, "fo_residual_rms_norm_bwd_workspace_bytes: bad argument");
-  *bytes = (M + (int64_t)3 * chunks_of(M) * N) * 4;
+  *bytes = ((M + 3) / 4 * 4 + 3 * partial_rows(M, N) * N) * 4;  // c2 of each row, partial rows
   return FO_OK;
 }
 
@@ -304,7 +734,7 @@ extern "C" int fo_residual_rms_norm_bwd(
   float* ws = (float*)workspace;
   const Bwd a{dout, dres, y, residual, weight, post_weight, gate, scale_vec, inv1, inv2, dy, dr,
               dgate, dw, post_weight ? dwp : nullptr, scale_vec ? ds : nullptr,
-              ws, ws + M, M, N, y_ld, r_ld, g_ld, scale, act};
+              ws, ws + (M + 3) / 4 * 4, M, N, y_ld, r_ld, g_ld, scale, act};
   return with_types(dtype, w_dtype, [&](auto t, auto w) {
     return run_bwd<decltype(t), decltype(w)>(a, st);
   });
