@@ -96,21 +96,14 @@ template <typename T, int V> struct Elem {
   using W = typename Word<kBytes>::type;
   using F = typename Lane<V>::F;
   static __device__ __forceinline__ F load(const void* p) {
-    const W w = *reinterpret_cast<const W*>(p);
-    const T* e = reinterpret_cast<const T*>(&w);
-    if constexpr (V == 1) return to_f<T>(e[0]);
-    else return make_float2(to_f<T>(e[0]), to_f<T>(e[1]));
+    if constexpr (V == 1) return to_f<T>(*reinterpret_cast<const T*>(p));
+    else if constexpr (sizeof(T) == 2) return unpack2<T>(*reinterpret_cast<const uint32_t*>(p));
+    else return *reinterpret_cast<const float2*>(p);
   }
   static __device__ __forceinline__ void store(T* p, F v) {
-    W w;
-    T* e = reinterpret_cast<T*>(&w);
-    if constexpr (V == 1) {
-      e[0] = from_f<T>(v);
-    } else {
-      e[0] = from_f<T>(v.x);
-      e[1] = from_f<T>(v.y);
-    }
-    *reinterpret_cast<W*>(p) = w;
+    if constexpr (V == 1) *p = from_f<T>(v);
+    else if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t*>(p) = pack2<T>(v);
+    else *reinterpret_cast<float2*>(p) = v;
   }
   static __device__ __forceinline__ void zero(void* smem) { *reinterpret_cast<W*>(smem) = W{}; }
   // global -> shared without waiting (2-byte elements have no such copy: through a register)

@@ -55,6 +55,24 @@ __device__ __forceinline__ float2 add_(float2 a, float2 b) {
       : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
   return d;
 }
+// A pair of T, as it is in memory, to and from fp32
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float2 f);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float2 f) {
+  const __nv_bfloat162 h = __float22bfloat162_rn(f);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float2 f) {
+  const __half2 h = __float22half2_rn(f);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 template <typename F> __device__ __forceinline__ F all_(float x);
 template <> __device__ __forceinline__ float all_<float>(float x) { return x; }
 template <> __device__ __forceinline__ float2 all_<float2>(float x) { return make_float2(x, x); }

@@ -70,26 +70,125 @@ __device__ __forceinline__ void act_grad(int act, float z, float& a, float& da) 
 }
 
 // ---------------------------------------------------------------------------
-// Rows in a shared-memory ring
+// A row in the threads that own it
 // ---------------------------------------------------------------------------
 template <int TPR> struct Shape {
-  static constexpr int kThreads = TPR > 256 ? TPR : TPR > 32 ? TPR : 256;
+  static constexpr int kThreads = TPR > 32 ? TPR : 256;
   static constexpr int kRows = kThreads / TPR;  // rows side by side in a CTA
 };
 
-// Streams [S] of rows in two stages; slot(s, k, i): vector i of stream k in stage s, of this thread.
-template <int S, int VPT, int THREADS> struct Ring {
-  uint4 v[2][S][VPT][THREADS];
-  __device__ __forceinline__ uint4& slot(int s, int k, int i) { return v[s][k][i][threadIdx.x]; }
-  __device__ __forceinline__ void fetch(int s, int k, int i, const void* p) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                     (uint32_t)__cvta_generic_to_shared(&slot(s, k, i))),
-                 "l"(p)
-                 : "memory");
+// What a thread has of a row: VPT vectors of E elements, TPR vectors apart, as fp32 pairs.
+// WIDE: vectors of 16 bytes, rows of S streams on their way in a ring of two stages in shared
+// memory.  Otherwise rows that 16-byte vectors do not fit: E = 2 elements TPR apart, read where
+// they are needed first into registers.
+template <typename T, typename W, int TPR, int VPT, bool WIDE, int S> struct Columns;
+
+template <typename T, typename W, int TPR, int VPT, int S>
+struct Columns<T, W, TPR, VPT, true, S> {
+  static constexpr int E = Vec16<T>::E, P = E / 2, kThreads = Shape<TPR>::kThreads;
+  static constexpr int kRingBytes = 2 * S * VPT * kThreads * 16;
+  uint4* ring;
+  int v0, nvec;
+  __device__ __forceinline__ Columns(uint8_t* smem, int64_t N)
+      : ring(reinterpret_cast<uint4*>(smem) + threadIdx.x), v0(threadIdx.x % TPR), nvec((int)(N / E)) {}
+  __device__ __forceinline__ uint4* slot(int stage, int k, int i) {
+    return ring + ((stage * S + k) * VPT + i) * kThreads;
+  }
+  __device__ __forceinline__ bool on(int i) const { return v0 + i * TPR < nvec; }
+  __device__ __forceinline__ void fetch(int stage, int k, const T* row) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      if (on(i))
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                         (uint32_t)__cvta_generic_to_shared(slot(stage, k, i))),
+                     "l"(row + (v0 + i * TPR) * E)
+                     : "memory");
+  }
+  __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  template <int LEFT> __device__ __forceinline__ void wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+  }
+  // A vector as it is in memory, pair q of it, and one filled with a number (exact in any type)
+  template <typename U> struct Words { uint4 u[E * (int)sizeof(U) / 16]; };
+  using Raw = Words<T>;
+  using RawW = Words<W>;
+  template <typename U> static __device__ __forceinline__ float2 pair(const Words<U>& r, int q) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(r.u);
+    if constexpr (sizeof(U) == 2) return unpack2<U>(w[q]);
+    else return make_float2(__uint_as_float(w[2 * q]), __uint_as_float(w[2 * q + 1]));
+  }
+  template <typename U> static __device__ __forceinline__ void set(Words<U>& r, int q, float2 f) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(r.u);
+    if constexpr (sizeof(U) == 2) {
+      w[q] = pack2<U>(f);
+    } else {
+      w[2 * q] = __float_as_uint(f.x);
+      w[2 * q + 1] = __float_as_uint(f.y);
+    }
+  }
+  template <typename U> static __device__ __forceinline__ Words<U> filled(float v) {
+    Words<U> r;
+#pragma unroll
+    for (int q = 0; q < P; ++q) set<U>(r, q, all_<float2>(v));
+    return r;
+  }
+  __device__ __forceinline__ Raw get(int stage, int k, int i) { return {{*slot(stage, k, i)}}; }
+  __device__ __forceinline__ RawW weights(const W* w, int i) const {
+    RawW r;
+#pragma unroll
+    for (int k = 0; k < E * (int)sizeof(W) / 16; ++k)
+      r.u[k] = ld_global_nc_v4(w + (v0 + i * TPR) * E + k * Vec16<W>::E);
+    return r;
+  }
+  __device__ __forceinline__ void put(T* row, int i, const Raw& r) const {
+    st_global_stream_v4(row + (v0 + i * TPR) * E, r.u[0]);
+  }
+  __device__ __forceinline__ void put_sums(float* row, int i, const float2 (&f)[P]) const {
+#pragma unroll
+    for (int q = 0; q < P; ++q) *reinterpret_cast<float2*>(row + (v0 + i * TPR) * E + 2 * q) = f[q];
   }
 };
-__device__ __forceinline__ void ring_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void ring_wait_one() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+
+template <typename T, typename W, int TPR, int VPT, int S>
+struct Columns<T, W, TPR, VPT, false, S> {
+  static constexpr int E = 2, P = 1, kThreads = Shape<TPR>::kThreads, kRingBytes = 0;
+  T raw[S][VPT][2];
+  int c0, N;
+  __device__ __forceinline__ Columns(uint8_t*, int64_t N_) : c0(threadIdx.x % TPR), N((int)N_) {}
+  __device__ __forceinline__ int at(int i, int e) const { return c0 + (2 * i + e) * TPR; }
+  __device__ __forceinline__ bool on(int i) const { return at(i, 0) < N; }
+  __device__ __forceinline__ void fetch(int, int k, const T* row) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) raw[k][i][e] = at(i, e) < N ? row[at(i, e)] : from_f<T>(0.f);
+  }
+  template <typename U> struct Words { U e[2]; };
+  using Raw = Words<T>;
+  using RawW = Words<W>;
+  template <typename U> static __device__ __forceinline__ float2 pair(const Words<U>& r, int) {
+    return make_float2(to_f<U>(r.e[0]), to_f<U>(r.e[1]));
+  }
+  template <typename U> static __device__ __forceinline__ void set(Words<U>& r, int, float2 f) {
+    r.e[0] = from_f<U>(f.x);
+    r.e[1] = from_f<U>(f.y);
+  }
+  template <typename U> static __device__ __forceinline__ Words<U> filled(float v) {
+    return {{from_f<U>(v), from_f<U>(v)}};
+  }
+  __device__ __forceinline__ Raw get(int, int k, int i) { return {{raw[k][i][0], raw[k][i][1]}}; }
+  __device__ __forceinline__ RawW weights(const W* w, int i) const {
+    return {{w[at(i, 0)], at(i, 1) < N ? w[at(i, 1)] : from_f<W>(0.f)}};
+  }
+  __device__ __forceinline__ void put(T* row, int i, const Raw& r) const {
+    row[at(i, 0)] = r.e[0];
+    if (at(i, 1) < N) row[at(i, 1)] = r.e[1];
+  }
+  __device__ __forceinline__ void put_sums(float* row, int i, const float2 (&f)[1]) const {
+    row[at(i, 0)] = f[0].x;
+    if (at(i, 1) < N) row[at(i, 1)] = f[0].y;
+  }
+};
 
 // Sums of K values over the TPR threads of a row, in every one of them.  `red`: [K][warps], not
 // used by the reduction before this one.
@@ -115,233 +214,239 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float (*red)[32]) {
   }
 }
 
-// f *= the weights' vector v (f *= number where there is none)
-template <typename W, int E>
-__device__ __forceinline__ void times(float (&f)[E], const W* w, int v, float number) {
-  if (w) {
-    float t[E];
-    constexpr int kPer = Vec16<W>::E;  // fp32 weights of 16-bit rows: two loads a vector
-#pragma unroll
-    for (int e = 0; e < E; e += kPer) unpack16<W>(ld_global_nc_v4(w + (int64_t)v * E + e), t + e);
-#pragma unroll
-    for (int e = 0; e < E; ++e) f[e] *= t[e];
-  } else {
-#pragma unroll
-    for (int e = 0; e < E; ++e) f[e] *= number;
-  }
+// sigmoid(z) and 1 - sigmoid(z) of pairs: e = e^-z, s = 1 / (1 + e), c = e s.  e is kept below
+// 2^126, so that e s is 1 (and s 1e-38 instead of 0) at the far end.
+__device__ __forceinline__ void sigmoid_pair(float2 z, float2& s, float2& c) {
+  const float2 e = map_([](float v) { return ex2(fminf(v, 126.f)); }, mul_(z, all_<float2>(-kLog2e)));
+  s = map_(rcp, add_(e, all_<float2>(1.f)));
+  c = mul_(e, s);
 }
 
-template <typename T, typename W, int TPR, int VPT>
+template <typename T, typename W, int TPR, int VPT, bool WIDE>
 __global__ void __launch_bounds__(Shape<TPR>::kThreads, 1024 / Shape<TPR>::kThreads)
 rrn_fwd_kernel(Fwd a) {
   using S = Shape<TPR>;
-  constexpr int E = Vec16<T>::E;
+  using C = Columns<T, W, TPR, VPT, WIDE, 3>;
+  constexpr int P = C::P;
   extern __shared__ __align__(16) uint8_t smem[];
-  auto& ring = *reinterpret_cast<Ring<3, VPT, S::kThreads>*>(smem);
   __shared__ float red[4][32];
   const W *w = (const W*)a.w, *wp = (const W*)a.wp, *sv = (const W*)a.sv;
-  const int nvec = (int)(a.N / E), v0 = threadIdx.x % TPR;
+  C col(smem, a.N);
   const float n = (float)a.N;
   const int64_t step = (int64_t)gridDim.x * S::kRows, mine = threadIdx.x / TPR;
-  auto fetch = [&](int64_t base, int s) {
+  auto fetch = [&](int64_t base, int stage) {
     const int64_t row = base + mine;
     if (row < a.M) {
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int v = v0 + i * TPR;
-        if (v < nvec) {
-          ring.fetch(s, 0, i, (const T*)a.y + row * a.y_ld + v * E);
-          ring.fetch(s, 1, i, (const T*)a.r + row * a.r_ld + v * E);
-          if (a.gate) ring.fetch(s, 2, i, (const T*)a.gate + row * a.g_ld + v * E);
-        }
-      }
+      col.fetch(stage, 0, (const T*)a.y + row * a.y_ld);
+      col.fetch(stage, 1, (const T*)a.r + row * a.r_ld);
+      if (a.gate) col.fetch(stage, 2, (const T*)a.gate + row * a.g_ld);
     }
-    ring_commit();
   };
   int64_t base = (int64_t)blockIdx.x * S::kRows;
-  fetch(base, 0);
+  if constexpr (WIDE) {
+    fetch(base, 0);
+    col.commit();
+  }
   for (int it = 0; base < a.M; base += step, ++it) {
     const int s = it & 1;
-    fetch(base + step, s ^ 1);
-    ring_wait_one();
+    if constexpr (WIDE) {
+      fetch(base + step, s ^ 1);
+      col.commit();
+      col.template wait<1>();
+    } else {
+      fetch(base, s);
+    }
     const int64_t row = base + mine;
     const bool on = row < a.M;
     float inv1 = 1.f;
     if (wp) {
-      float ss[1] = {0.f};
+      float2 ss = all_<float2>(0.f);
 #pragma unroll
       for (int i = 0; i < VPT; ++i)
-        if (on && v0 + i * TPR < nvec) {
-          float f[E];
-          unpack16<T>(ring.slot(s, 0, i), f);
+        if (on && col.on(i)) {
+          const auto y = col.get(s, 0, i);
 #pragma unroll
-          for (int e = 0; e < E; ++e) ss[0] = fmaf(f[e], f[e], ss[0]);
+          for (int q = 0; q < P; ++q) ss = fma_(C::pair(y, q), C::pair(y, q), ss);
         }
-      row_sum<TPR>(ss, red + s);
-      inv1 = 1.f / sqrtf(ss[0] / n + a.eps);
+      float sum[1] = {ss.x + ss.y};
+      row_sum<TPR>(sum, red + s);
+      inv1 = 1.f / sqrtf(sum[0] / n + a.eps);
     }
-    float r2[VPT][E], ss[1] = {0.f};
+    float2 r2[VPT][P], ss = all_<float2>(0.f);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int v = v0 + i * TPR;
-      if (on && v < nvec) {
-        float u[E];
-        unpack16<T>(ring.slot(s, 0, i), u);
+      if (on && col.on(i)) {
+        const auto y = col.get(s, 0, i), r = col.get(s, 1, i);
+        float2 u[P];
 #pragma unroll
-        for (int e = 0; e < E; ++e) u[e] *= inv1;
-        if (wp) times<W>(u, wp, v, 1.f);
+        for (int q = 0; q < P; ++q) u[q] = mul_(C::pair(y, q), all_<float2>(inv1));
+        if (wp) {
+          const auto t = col.weights(wp, i);
+#pragma unroll
+          for (int q = 0; q < P; ++q) u[q] = mul_(u[q], C::pair(t, q));
+        }
         if (a.gate) {
-          float z[E];
-          unpack16<T>(ring.slot(s, 2, i), z);
+          const auto z = col.get(s, 2, i);
 #pragma unroll
-          for (int e = 0; e < E; ++e) u[e] *= act_of(a.act, z[e]);
+          for (int q = 0; q < P; ++q) {
+            const float2 e = map_(ex2, mul_(C::pair(z, q), all_<float2>(-kLog2e)));
+            u[q] = mul_(u[q], map_(rcp, add_(e, all_<float2>(1.f))));
+            if (a.act == FO_ACT_SILU) u[q] = mul_(u[q], C::pair(z, q));
+          }
         }
-        times<W>(u, sv, v, a.s);
-        float r[E];
-        unpack16<T>(ring.slot(s, 1, i), r);
+        if (sv) {
+          const auto t = col.weights(sv, i);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          r2[i][e] = r[e] + u[e];
-          ss[0] = fmaf(r2[i][e], r2[i][e], ss[0]);
+          for (int q = 0; q < P; ++q) r2[i][q] = fma_(u[q], C::pair(t, q), C::pair(r, q));
+        } else {
+#pragma unroll
+          for (int q = 0; q < P; ++q) r2[i][q] = fma_(u[q], all_<float2>(a.s), C::pair(r, q));
         }
+#pragma unroll
+        for (int q = 0; q < P; ++q) ss = fma_(r2[i][q], r2[i][q], ss);
       }
     }
-    row_sum<TPR>(ss, red + 2 + s);
-    const float inv2 = 1.f / sqrtf(ss[0] / n + a.eps);
-    if (on && v0 == 0) {
+    float sum[1] = {ss.x + ss.y};
+    row_sum<TPR>(sum, red + 2 + s);
+    const float inv2 = 1.f / sqrtf(sum[0] / n + a.eps);
+    if (on && threadIdx.x % TPR == 0) {
       if (a.inv1) a.inv1[row] = inv1;
       if (a.inv2) a.inv2[row] = inv2;
     }
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int v = v0 + i * TPR;
-      if (on && v < nvec) {
-        st_global_stream_v4((T*)a.res + row * a.N + v * E, pack16<T>(r2[i]));
+      if (on && col.on(i)) {
+        const auto t = col.weights(w, i);
+        typename C::Raw res, out;
 #pragma unroll
-        for (int e = 0; e < E; ++e) r2[i][e] *= inv2;
-        times<W>(r2[i], w, v, 1.f);
-        st_global_stream_v4((T*)a.out + row * a.N + v * E, pack16<T>(r2[i]));
+        for (int q = 0; q < P; ++q) {
+          C::set(res, q, r2[i][q]);
+          C::set(out, q, mul_(mul_(r2[i][q], all_<float2>(inv2)), C::pair(t, q)));
+        }
+        col.put((T*)a.res + row * a.N, i, res);
+        col.put((T*)a.out + row * a.N, i, out);
       }
     }
   }
 }
 
-template <typename T, typename W, int TPR, int VPT>
+template <typename T, typename W, int TPR, int VPT, bool WIDE>
 __global__ void __launch_bounds__(Shape<TPR>::kThreads, 512 / Shape<TPR>::kThreads)
 rrn_bwd_kernel(Bwd a) {
   using S = Shape<TPR>;
-  constexpr int E = Vec16<T>::E;
+  using C = Columns<T, W, TPR, VPT, WIDE, 5>;
+  constexpr int P = C::P;
   extern __shared__ __align__(16) uint8_t smem[];
-  auto& ring = *reinterpret_cast<Ring<5, VPT, S::kThreads>*>(smem);
   __shared__ float red[6][32];
   const W *w = (const W*)a.w, *wp = (const W*)a.wp, *sv = (const W*)a.sv;
-  const int nvec = (int)(a.N / E), v0 = threadIdx.x % TPR;
+  C col(smem, a.N);
   const int64_t step = (int64_t)gridDim.x * S::kRows, mine = threadIdx.x / TPR;
-  auto fetch = [&](int64_t base, int s) {
+  auto fetch = [&](int64_t base, int stage) {
     const int64_t row = base + mine;
     if (row < a.M) {
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int v = v0 + i * TPR;
-        if (v < nvec) {
-          ring.fetch(s, 0, i, (const T*)a.y + row * a.y_ld + v * E);
-          ring.fetch(s, 1, i, (const T*)a.r + row * a.r_ld + v * E);
-          if (a.gate) ring.fetch(s, 2, i, (const T*)a.gate + row * a.g_ld + v * E);
-          if (a.dout) ring.fetch(s, 3, i, (const T*)a.dout + row * a.N + v * E);
-          if (a.dres) ring.fetch(s, 4, i, (const T*)a.dres + row * a.N + v * E);
-        }
-      }
+      col.fetch(stage, 0, (const T*)a.y + row * a.y_ld);
+      col.fetch(stage, 1, (const T*)a.r + row * a.r_ld);
+      if (a.gate) col.fetch(stage, 2, (const T*)a.gate + row * a.g_ld);
+      if (a.dout) col.fetch(stage, 3, (const T*)a.dout + row * a.N);
+      if (a.dres) col.fetch(stage, 4, (const T*)a.dres + row * a.N);
     }
-    ring_commit();
   };
-  // Of a vector: y, p / inv1 = y w_post, act and act', s, r', d, e, dr'
+  // A vector of every input.  What is absent is filled in, so that the arithmetic has no branches:
+  // w_post with 1, a gate with 100 (its sigmoid is 1), gradients with 0.
+  const bool silu = a.act == FO_ACT_SILU;
   struct Part {
-    float y[E], q[E], av[E], da[E], sj[E], r2[E], d[E], e[E], dr[E];
+    typename C::Raw y, r, z, d, dr;
+    typename C::RawW w, wp, sv;
   };
-  auto load = [&](int s, int i, int v, float inv1, Part& p) {
-    unpack16<T>(ring.slot(s, 0, i), p.y);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      p.q[e] = p.y[e];
-      p.sj[e] = 1.f;
-      p.av[e] = 1.f;
-      p.da[e] = 0.f;
-      p.d[e] = p.dr[e] = 0.f;
-    }
-    if (wp) times<W>(p.q, wp, v, 1.f);
-    times<W>(p.sj, sv, v, a.s);
-    if (a.gate) {
-      float z[E];
-      unpack16<T>(ring.slot(s, 2, i), z);
-#pragma unroll
-      for (int e = 0; e < E; ++e) act_grad(a.act, z[e], p.av[e], p.da[e]);
-    }
-    unpack16<T>(ring.slot(s, 1, i), p.r2);
-#pragma unroll
-    for (int e = 0; e < E; ++e) p.r2[e] = fmaf(p.sj[e] * p.av[e], inv1 * p.q[e], p.r2[e]);
-    if (a.dout) unpack16<T>(ring.slot(s, 3, i), p.d);
-#pragma unroll
-    for (int e = 0; e < E; ++e) p.e[e] = p.d[e];
-    times<W>(p.e, w, v, 1.f);
-    if (a.dres) unpack16<T>(ring.slot(s, 4, i), p.dr);
+  auto load = [&](int s, int i, Part& p) {
+    p.y = col.get(s, 0, i);
+    p.r = col.get(s, 1, i);
+    p.z = a.gate ? col.get(s, 2, i) : C::template filled<T>(100.f);
+    p.d = a.dout ? col.get(s, 3, i) : C::template filled<T>(0.f);
+    p.dr = a.dres ? col.get(s, 4, i) : C::template filled<T>(0.f);
+    p.w = col.weights(w, i);
+    p.wp = wp ? col.weights(wp, i) : C::template filled<W>(1.f);
+    if (sv) p.sv = col.weights(sv, i);
   };
-  float dw[VPT][E], ds[VPT][E], dwp[VPT][E];
+  auto scale_of = [&](const Part& p, int q) { return sv ? C::pair(p.sv, q) : all_<float2>(a.s); };
+  float2 dw[VPT][P], ds[VPT][P], dwp[VPT][P];
 #pragma unroll
   for (int i = 0; i < VPT; ++i)
 #pragma unroll
-    for (int e = 0; e < E; ++e) dw[i][e] = ds[i][e] = dwp[i][e] = 0.f;
+    for (int q = 0; q < P; ++q) dw[i][q] = ds[i][q] = dwp[i][q] = all_<float2>(0.f);
   int64_t base = (int64_t)blockIdx.x * S::kRows;
-  fetch(base, 0);
+  if constexpr (WIDE) {
+    fetch(base, 0);
+    col.commit();
+  }
   for (int it = 0; base < a.M; base += step, ++it) {
     const int s = it & 1;
-    fetch(base + step, s ^ 1);
+    if constexpr (WIDE) {
+      fetch(base + step, s ^ 1);
+      col.commit();
+    } else {
+      fetch(base, s);
+    }
     const int64_t row = base + mine;
     const bool on = row < a.M;
     const float inv1 = wp && on ? a.inv1[row] : 1.f, inv2 = on ? a.inv2[row] : 1.f;
-    ring_wait_one();
-    float sum[3] = {0.f, 0.f, 0.f};
+    const float2 i1 = all_<float2>(inv1), i2 = all_<float2>(inv2);
+    if constexpr (WIDE) col.template wait<1>();
+    float2 s1 = all_<float2>(0.f), s2 = s1, s3 = s1;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int v = v0 + i * TPR;
-      if (on && v < nvec) {
+      if (on && col.on(i)) {
         Part p;
-        load(s, i, v, inv1, p);
+        load(s, i, p);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float qy = p.sj[e] * p.av[e] * p.q[e];
-          sum[0] = fmaf(p.e[e], p.r2[e], sum[0]);
-          sum[1] = fmaf(qy, fmaf(inv2, p.e[e], p.dr[e]), sum[1]);
-          sum[2] = fmaf(qy, p.r2[e], sum[2]);
+        for (int q = 0; q < P; ++q) {
+          const float2 z = C::pair(p.z, q);
+          float2 av, c;
+          sigmoid_pair(z, av, c);
+          if (silu) av = mul_(av, z);
+          const float2 qy = mul_(mul_(scale_of(p, q), av), mul_(C::pair(p.y, q), C::pair(p.wp, q)));
+          const float2 r2 = fma_(i1, qy, C::pair(p.r, q));
+          const float2 e = mul_(C::pair(p.d, q), C::pair(p.w, q));
+          s1 = fma_(e, r2, s1);
+          s2 = fma_(qy, fma_(i2, e, C::pair(p.dr, q)), s2);
+          s3 = fma_(qy, r2, s3);
         }
       }
     }
+    float sum[3] = {s1.x + s1.y, s2.x + s2.y, s3.x + s3.y};
     row_sum<TPR>(sum, red + 3 * s);
     const float c2 = inv2 * inv2 * inv2 * sum[0] / (float)a.N;
     const float c1 = wp ? inv1 * inv1 * inv1 * fmaf(-c2, sum[2], sum[1]) / (float)a.N : 0.f;
+    const float2 m2 = all_<float2>(-c2), m1 = all_<float2>(-c1);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int v = v0 + i * TPR;
-      if (on && v < nvec) {
+      if (on && col.on(i)) {
         Part p;
-        load(s, i, v, inv1, p);
-        float dr[E], dy[E], dg[E], k[E];
+        load(s, i, p);
+        typename C::Raw dr, dy, dg;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float D = fmaf(inv2, p.e[e], fmaf(-c2, p.r2[e], p.dr[e]));
-          const float pe = p.q[e] * inv1, sD = p.sj[e] * D;
-          dr[e] = D;
-          dg[e] = sD * pe * p.da[e];
-          k[e] = sD * p.av[e];
-          dw[i][e] = fmaf(p.d[e] * p.r2[e], inv2, dw[i][e]);
-          ds[i][e] = fmaf(D, p.av[e] * pe, ds[i][e]);
-          dwp[i][e] = fmaf(k[e], p.y[e] * inv1, dwp[i][e]);
+        for (int q = 0; q < P; ++q) {
+          const float2 z = C::pair(p.z, q), wq = C::pair(p.wp, q), sj = scale_of(p, q);
+          const float2 n = mul_(C::pair(p.y, q), i1), pe = mul_(n, wq);
+          float2 sg, c;
+          sigmoid_pair(z, sg, c);
+          const float2 av = silu ? mul_(sg, z) : sg;
+          const float2 u = mul_(av, pe), r2 = fma_(sj, u, C::pair(p.r, q));
+          const float2 d = C::pair(p.d, q), e = mul_(d, C::pair(p.w, q));
+          const float2 D = fma_(i2, e, fma_(m2, r2, C::pair(p.dr, q))), sD = mul_(sj, D);
+          // silu' = s (1 + z c), sigmoid' = s c
+          const float2 f = silu ? fma_(z, c, all_<float2>(1.f)) : c;
+          const float2 dp = mul_(sD, av);
+          C::set(dr, q, D);
+          C::set(dg, q, mul_(mul_(sD, pe), mul_(sg, f)));
+          C::set(dy, q, fma_(i1, mul_(dp, wq), mul_(m1, C::pair(p.y, q))));
+          dw[i][q] = fma_(mul_(d, i2), r2, dw[i][q]);
+          ds[i][q] = fma_(D, u, ds[i][q]);
+          dwp[i][q] = fma_(dp, n, dwp[i][q]);
         }
-        if (wp) times<W>(k, wp, v, 1.f);
-#pragma unroll
-        for (int e = 0; e < E; ++e) dy[e] = fmaf(inv1, k[e], -c1 * p.y[e]);
-        st_global_stream_v4((T*)a.dr + row * a.N + v * E, pack16<T>(dr));
-        st_global_stream_v4((T*)a.dy + row * a.N + v * E, pack16<T>(dy));
-        if (a.gate) st_global_stream_v4((T*)a.dgate + row * a.N + v * E, pack16<T>(dg));
+        col.put((T*)a.dr + row * a.N, i, dr);
+        col.put((T*)a.dy + row * a.N, i, dy);
+        if (a.gate) col.put((T*)a.dgate + row * a.N, i, dg);
       }
     }
   }
@@ -350,33 +455,25 @@ rrn_bwd_kernel(Bwd a) {
   float* part = a.part + (int64_t)blockIdx.x * a.N;
   if constexpr (S::kRows == 1) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int v = v0 + i * TPR;
-      if (v < nvec)
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          part[v * E + e] = dw[i][e];
-          part[stride + v * E + e] = ds[i][e];
-          part[2 * stride + v * E + e] = dwp[i][e];
-        }
-    }
+    for (int i = 0; i < VPT; ++i)
+      if (col.on(i)) {
+        col.put_sums(part, i, dw[i]);
+        col.put_sums(part + stride, i, ds[i]);
+        col.put_sums(part + 2 * stride, i, dwp[i]);
+      }
   } else {
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if constexpr (WIDE) col.template wait<0>();
     float* sums = reinterpret_cast<float*>(smem);  // [rows][3][N], over the ring
     __syncthreads();
     const int N = (int)a.N;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int v = v0 + i * TPR;
-      if (v < nvec)
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          float* to = sums + mine * 3 * N + v * E + e;
-          to[0] = dw[i][e];
-          to[N] = ds[i][e];
-          to[2 * N] = dwp[i][e];
-        }
-    }
+    for (int i = 0; i < VPT; ++i)
+      if (col.on(i)) {
+        float* to = sums + mine * 3 * N;
+        col.put_sums(to, i, dw[i]);
+        col.put_sums(to + N, i, ds[i]);
+        col.put_sums(to + 2 * N, i, dwp[i]);
+      }
     __syncthreads();
     for (int j = threadIdx.x; j < 3 * N; j += S::kThreads) {
       float t = 0.f;
@@ -552,35 +649,49 @@ int64_t partial_rows(int64_t M, int64_t N) {
   return g < M ? g : (M > 0 ? M : 1);
 }
 
-template <typename T, typename W> constexpr int kMostVectors = 1024;
-
-// Calls f(TPR, VPT) with the smallest shape whose threads cover nvec vectors: a warp or less for
-// the narrowest rows (no barrier), else a CTA of up to 512 threads with one or two vectors each.
-template <typename F> int with_shape(int64_t nvec, F&& f) {
-  auto go = [&](auto tpr, auto vpt) { return f(tpr, vpt); };
+// Calls f(TPR, VPT, WIDE) with the smallest shape whose threads cover a row of N elements: a warp or
+// less for the narrowest rows (no barrier), else a CTA of up to 512 threads.  Returns -1 where
+// none does.
+template <typename T, typename F> int with_shape(bool wide, int64_t N, F&& f) {
   using std::integral_constant;
-  if (nvec <= 8) return go(integral_constant<int, 8>{}, integral_constant<int, 1>{});
-  if (nvec <= 32) return go(integral_constant<int, 32>{}, integral_constant<int, 1>{});
-  if (nvec <= 64) return go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-  if (nvec <= 128) return go(integral_constant<int, 128>{}, integral_constant<int, 1>{});
-  if (nvec <= 256) return go(integral_constant<int, 256>{}, integral_constant<int, 1>{});
-  if (nvec <= 512) return go(integral_constant<int, 512>{}, integral_constant<int, 1>{});
-  return go(integral_constant<int, 512>{}, integral_constant<int, 2>{});
+  auto go = [&](auto tpr, auto vpt, auto w) {
+    return f(integral_constant<int, tpr>{}, integral_constant<int, vpt>{}, w);
+  };
+#define FO_SHAPE(TPR, VPT, PER, W) \
+  if (N <= (int64_t)TPR * VPT * PER) return go(integral_constant<int, TPR>{}, integral_constant<int, VPT>{}, W{})
+  if (wide) {
+    constexpr int E = Vec16<T>::E;
+    FO_SHAPE(8, 1, E, std::true_type);
+    FO_SHAPE(32, 1, E, std::true_type);
+    FO_SHAPE(64, 1, E, std::true_type);
+    FO_SHAPE(128, 1, E, std::true_type);
+    FO_SHAPE(256, 1, E, std::true_type);
+    FO_SHAPE(512, 1, E, std::true_type);
+    FO_SHAPE(512, 2, E, std::true_type);
+  } else {
+    FO_SHAPE(32, 1, 2, std::false_type);
+    FO_SHAPE(32, 4, 2, std::false_type);
+    FO_SHAPE(128, 4, 2, std::false_type);
+    FO_SHAPE(256, 4, 2, std::false_type);
+    FO_SHAPE(512, 4, 2, std::false_type);
+  }
+#undef FO_SHAPE
+  return -1;
 }
 
-template <typename T, typename W>
-bool ring_ok(int64_t N, const void* const* rows, const int64_t* lds, int n,
+template <typename T>
+bool wide_ok(int64_t N, const void* const* rows, const int64_t* lds, int n,
              const void* const* vectors, int nv) {
   constexpr int E = Vec16<T>::E;
-  bool ok = N % E == 0 && N / E <= kMostVectors<T, W>;
+  bool ok = N % E == 0;
   for (int i = 0; i < n; ++i) ok = ok && aligned16(rows[i]) && lds[i] % E == 0;
   for (int i = 0; i < nv; ++i) ok = ok && aligned16(vectors[i]);
   return ok;
 }
 
 template <typename K, typename A>
-int launch_ring(const char* what, K kernel, int64_t ctas, int threads, int smem, const A& a,
-                cudaStream_t st) {
+int launch(const char* what, K kernel, int64_t ctas, int threads, int smem, const A& a,
+           cudaStream_t st) {
   if (smem > 40 * 1024) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) {
@@ -603,15 +714,15 @@ template <typename T, typename W>
 int run_fwd(const Fwd& a, cudaStream_t st) {
   const void *rows[] = {a.y, a.r, a.gate, a.out, a.res}, *vs[] = {a.w, a.wp, a.sv};
   const int64_t lds[] = {a.y_ld, a.r_ld, a.g_ld, a.N, a.N};
-  if (ring_ok<T, W>(a.N, rows, lds, 5, vs, 3))
-    return with_shape(a.N / Vec16<T>::E, [&](auto tpr, auto vpt) {
-      using S = Shape<tpr>;
-      constexpr int smem = (int)sizeof(Ring<3, vpt, S::kThreads>);
-      const int64_t most = num_sms() * resident(1024, S::kThreads, smem);
-      const int64_t need = (a.M + S::kRows - 1) / S::kRows;
-      return launch_ring("rrn_fwd_kernel", rrn_fwd_kernel<T, W, tpr, vpt>,
-                         need < most ? need : most, S::kThreads, smem, a, st);
-    });
+  const int rc = with_shape<T>(wide_ok<T>(a.N, rows, lds, 5, vs, 3), a.N, [&](auto tpr, auto vpt, auto wide) {
+    using S = Shape<tpr>;
+    constexpr int smem = Columns<T, W, tpr, vpt, wide, 3>::kRingBytes;
+    const int64_t most = num_sms() * resident(1024, S::kThreads, smem);
+    const int64_t need = (a.M + S::kRows - 1) / S::kRows;
+    return launch("rrn_fwd_kernel", rrn_fwd_kernel<T, W, tpr, vpt, wide>, need < most ? need : most,
+                  S::kThreads, smem, a, st);
+  });
+  if (rc != -1) return rc;
   rrn_fwd_generic_kernel<T, W><<<row_grid(a.M), 256, 0, st>>>(a);
   return check_launch("rrn_fwd_generic_kernel");
 }
@@ -622,28 +733,26 @@ int run_bwd(const Bwd& a, cudaStream_t st) {
              *vs[] = {a.w, a.wp, a.sv};
   const int64_t lds[] = {a.y_ld, a.r_ld, a.g_ld, a.N, a.N, a.N, a.N, a.N};
   int G = 0;
-  if (ring_ok<T, W>(a.N, rows, lds, 8, vs, 3)) {
-    const int rc = with_shape(a.N / Vec16<T>::E, [&](auto tpr, auto vpt) {
-      using S = Shape<tpr>;
-      constexpr int ring = (int)sizeof(Ring<5, vpt, S::kThreads>);
-      const int sums = S::kRows > 1 ? (int)(S::kRows * 3 * a.N * 4) : 0;
-      const int smem = ring > sums ? ring : sums;
-      int64_t ctas = num_sms() * resident(512, S::kThreads, smem);
-      const int64_t need = (a.M + S::kRows - 1) / S::kRows, most = partial_rows(a.M, a.N);
-      if (ctas > need) ctas = need;
-      if (ctas > most) ctas = most;
-      G = (int)ctas;
-      return launch_ring("rrn_bwd_kernel", rrn_bwd_kernel<T, W, tpr, vpt>, ctas, S::kThreads, smem,
-                         a, st);
-    });
-    if (rc) return rc;
-  } else {
+  int rc = with_shape<T>(wide_ok<T>(a.N, rows, lds, 8, vs, 3), a.N, [&](auto tpr, auto vpt, auto wide) {
+    using S = Shape<tpr>;
+    constexpr int ring = Columns<T, W, tpr, vpt, wide, 5>::kRingBytes;
+    const int sums = S::kRows > 1 ? (int)(S::kRows * 3 * a.N * 4) : 0;
+    const int smem = ring > sums ? ring : sums;
+    int64_t ctas = num_sms() * resident(512, S::kThreads, smem);
+    const int64_t need = (a.M + S::kRows - 1) / S::kRows, most = partial_rows(a.M, a.N);
+    if (ctas > need) ctas = need;
+    if (ctas > most) ctas = most;
+    G = (int)ctas;
+    return launch("rrn_bwd_kernel", rrn_bwd_kernel<T, W, tpr, vpt, wide>, ctas, S::kThreads, smem, a, st);
+  });
+  if (rc == -1) {
     rrn_bwd_generic_kernel<T, W><<<row_grid(a.M), 256, 0, st>>>(a);
-    if (int rc = check_launch("rrn_bwd_generic_kernel")) return rc;
+    if (int e = check_launch("rrn_bwd_generic_kernel")) return e;
     G = (int)(a.M < kChunks ? a.M : kChunks);
     rrn_cols_kernel<T, W><<<dim3((unsigned)((a.N + 255) / 256), G), 256, 0, st>>>(a);
-    if (int rc = check_launch("rrn_cols_kernel")) return rc;
+    rc = check_launch("rrn_cols_kernel");
   }
+  if (rc) return rc;
   rrn_reduce_kernel<W><<<dim3((unsigned)((a.N + 31) / 32), 3), 32 * kReduceWarps, 0, st>>>(a, G);
   return check_launch("rrn_reduce_kernel");
 }
