@@ -7,9 +7,8 @@
 //
 // Backward from d = dL/dout and dr' = dL/dr', with e = d * w:
 //   D  = dr' + inv2 e - r' inv2^3 mean(e r')        (all that reaches r')
-//   dr = D,  ds = sum D u,  dw = sum d r' inv2
-//   dgate = s D p act'(gate),  dp = s D act(gate)
-//   dw_post = sum dp y inv1,  k = dp w_post,  dy = inv1 k - y inv1^3 mean(k y)
+//   dr = D,  dw = sum d r' inv2,  A = sum D act(gate) y inv1,  ds = w_post A,  dw_post = s A
+//   dgate = s D p act'(gate),  k = s w_post D act(gate),  dy = inv1 k - y inv1^3 mean(k y)
 // r' is recomputed from y, gate, r and the forward's inv1, inv2 in fp32, so gradients do not see
 // the rounding of the stored r'.  mean(k y) needs D, which needs mean(e r'); writing
 //   sum k y = sum q y (dr' + inv2 e) - c2 sum q y r',  q = s act w_post, c2 = inv2^3 mean(e r')
@@ -19,9 +18,12 @@
 // 16-byte vectors each, and CTAs walk over the rows: every input is read once, by cp.async into a
 // ring of two rows in shared memory (the next row is on its way while this one is reduced and
 // written), and a thread only ever reads the slots that it filled, so the ring needs no barrier.
-// The backward keeps its threads' column sums in registers over all rows of the CTA, writes them
-// as one partial row a CTA, and a column kernel adds those up in their order.  Other widths take
-// the generic kernels: several passes over the row, through L1 and L2.
+// The backward keeps its threads' column sums (of dw and A) in registers over all rows of the CTA,
+// writes them as one partial row a CTA, and a column kernel adds those up in their order; s w_post
+// and w are kept in shared memory in fp32.  Its arithmetic is what limits it next (a sigmoid and some
+// thirty operations an element), so it is done on pairs.  Rows that 16-byte vectors do not fit are
+// read into registers instead; wider rows take the generic kernels: several passes over the row,
+// through L1 and L2.
 #include <type_traits>
 
 #include "gates.cuh"
@@ -95,13 +97,16 @@ struct Columns<T, W, TPR, VPT, true, S> {
     return ring + ((stage * S + k) * VPT + i) * kThreads;
   }
   __device__ __forceinline__ bool on(int i) const { return v0 + i * TPR < nvec; }
-  __device__ __forceinline__ void fetch(int stage, int k, const T* row) {
+  // Bytes from a row's begin to this thread's first element
+  __device__ __forceinline__ int64_t first() const { return v0 * 16; }
+  // p: a row's begin plus first()
+  __device__ __forceinline__ void fetch(int stage, int k, const uint8_t* p) {
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(slot(stage, k, 0));
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
       if (on(i))
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                         (uint32_t)__cvta_generic_to_shared(slot(stage, k, i))),
-                     "l"(row + (v0 + i * TPR) * E)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i * kThreads * 16),
+                     "l"(p + i * TPR * 16)
                      : "memory");
   }
   __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -140,8 +145,17 @@ struct Columns<T, W, TPR, VPT, true, S> {
       r.u[k] = ld_global_nc_v4(w + (v0 + i * TPR) * E + k * Vec16<W>::E);
     return r;
   }
-  __device__ __forceinline__ void put(T* row, int i, const Raw& r) const {
-    st_global_stream_v4(row + (v0 + i * TPR) * E, r.u[0]);
+  // Of fp32 weights in shared memory
+  __device__ __forceinline__ void weights(const float* smem, int i, float2 (&f)[P]) const {
+#pragma unroll
+    for (int q = 0; q < P; q += 2) {
+      const float4 v = *reinterpret_cast<const float4*>(smem + (v0 + i * TPR) * E + 2 * q);
+      f[q] = make_float2(v.x, v.y);
+      f[q + 1] = make_float2(v.z, v.w);
+    }
+  }
+  __device__ __forceinline__ void put(uint8_t* p, int i, const Raw& r) const {
+    st_global_stream_v4(p + i * TPR * 16, r.u[0]);
   }
   __device__ __forceinline__ void put_sums(float* row, int i, const float2 (&f)[P]) const {
 #pragma unroll
@@ -157,11 +171,13 @@ struct Columns<T, W, TPR, VPT, false, S> {
   __device__ __forceinline__ Columns(uint8_t*, int64_t N_) : c0(threadIdx.x % TPR), N((int)N_) {}
   __device__ __forceinline__ int at(int i, int e) const { return c0 + (2 * i + e) * TPR; }
   __device__ __forceinline__ bool on(int i) const { return at(i, 0) < N; }
-  __device__ __forceinline__ void fetch(int, int k, const T* row) {
+  __device__ __forceinline__ int64_t first() const { return c0 * (int)sizeof(T); }
+  __device__ __forceinline__ void fetch(int, int k, const uint8_t* p) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) raw[k][i][e] = at(i, e) < N ? row[at(i, e)] : from_f<T>(0.f);
+      for (int e = 0; e < 2; ++e)
+        raw[k][i][e] = at(i, e) < N ? reinterpret_cast<const T*>(p)[(2 * i + e) * TPR] : from_f<T>(0.f);
   }
   template <typename U> struct Words { U e[2]; };
   using Raw = Words<T>;
@@ -180,9 +196,12 @@ struct Columns<T, W, TPR, VPT, false, S> {
   __device__ __forceinline__ RawW weights(const W* w, int i) const {
     return {{w[at(i, 0)], at(i, 1) < N ? w[at(i, 1)] : from_f<W>(0.f)}};
   }
-  __device__ __forceinline__ void put(T* row, int i, const Raw& r) const {
-    row[at(i, 0)] = r.e[0];
-    if (at(i, 1) < N) row[at(i, 1)] = r.e[1];
+  __device__ __forceinline__ void weights(const float* smem, int i, float2 (&f)[1]) const {
+    f[0] = make_float2(smem[at(i, 0)], at(i, 1) < N ? smem[at(i, 1)] : 0.f);
+  }
+  __device__ __forceinline__ void put(uint8_t* p, int i, const Raw& r) const {
+    reinterpret_cast<T*>(p)[2 * i * TPR] = r.e[0];
+    if (at(i, 1) < N) reinterpret_cast<T*>(p)[(2 * i + 1) * TPR] = r.e[1];
   }
   __device__ __forceinline__ void put_sums(float* row, int i, const float2 (&f)[1]) const {
     row[at(i, 0)] = f[0].x;
@@ -222,6 +241,9 @@ __device__ __forceinline__ void sigmoid_pair(float2 z, float2& s, float2& c) {
   c = mul_(e, s);
 }
 
+// Bytes of two fp32 weight vectors of N elements, each a multiple of 16.
+__host__ __device__ constexpr int weight_bytes(int64_t N) { return (int)((N + 3) / 4 * 4 * 8); }
+
 template <typename T, typename W, int TPR, int VPT, bool WIDE>
 __global__ void __launch_bounds__(Shape<TPR>::kThreads, 1024 / Shape<TPR>::kThreads)
 rrn_fwd_kernel(Fwd a) {
@@ -234,29 +256,38 @@ rrn_fwd_kernel(Fwd a) {
   C col(smem, a.N);
   const float n = (float)a.N;
   const int64_t step = (int64_t)gridDim.x * S::kRows, mine = threadIdx.x / TPR;
-  auto fetch = [&](int64_t base, int stage) {
-    const int64_t row = base + mine;
-    if (row < a.M) {
-      col.fetch(stage, 0, (const T*)a.y + row * a.y_ld);
-      col.fetch(stage, 1, (const T*)a.r + row * a.r_ld);
-      if (a.gate) col.fetch(stage, 2, (const T*)a.gate + row * a.g_ld);
-    }
-  };
   int64_t base = (int64_t)blockIdx.x * S::kRows;
+  // what is fetched next, and what is written: the thread's first bytes of its row
+  const int64_t z = sizeof(T), r0 = base + mine;
+  const uint8_t *py = (const uint8_t*)a.y + r0 * a.y_ld * z + col.first(),
+                *pr = (const uint8_t*)a.r + r0 * a.r_ld * z + col.first(),
+                *pg = (const uint8_t*)a.gate + r0 * a.g_ld * z + col.first();
+  const int64_t dy = step * a.y_ld * z, dr = step * a.r_ld * z, dg = step * a.g_ld * z;
+  int64_t to = r0 * a.N * z + col.first();
+  auto fetch = [&](int64_t row, int stage) {
+    if (row < a.M) {
+      col.fetch(stage, 0, py);
+      col.fetch(stage, 1, pr);
+      if (a.gate) col.fetch(stage, 2, pg);
+    }
+    py += dy;
+    pr += dr;
+    pg += dg;
+  };
   if constexpr (WIDE) {
-    fetch(base, 0);
+    fetch(base + mine, 0);
     col.commit();
   }
-  for (int it = 0; base < a.M; base += step, ++it) {
+  for (int it = 0; base < a.M; base += step, to += step * a.N * z, ++it) {
     const int s = it & 1;
+    const int64_t row = base + mine;
     if constexpr (WIDE) {
-      fetch(base + step, s ^ 1);
+      fetch(row + step, s ^ 1);
       col.commit();
       col.template wait<1>();
     } else {
-      fetch(base, s);
+      fetch(row, s);
     }
-    const int64_t row = base + mine;
     const bool on = row < a.M;
     float inv1 = 1.f;
     if (wp) {
@@ -323,8 +354,8 @@ rrn_fwd_kernel(Fwd a) {
           C::set(res, q, r2[i][q]);
           C::set(out, q, mul_(mul_(r2[i][q], all_<float2>(inv2)), C::pair(t, q)));
         }
-        col.put((T*)a.res + row * a.N, i, res);
-        col.put((T*)a.out + row * a.N, i, out);
+        col.put((uint8_t*)a.res + to, i, res);
+        col.put((uint8_t*)a.out + to, i, out);
       }
     }
   }
@@ -335,28 +366,47 @@ __global__ void __launch_bounds__(Shape<TPR>::kThreads, 512 / Shape<TPR>::kThrea
 rrn_bwd_kernel(Bwd a) {
   using S = Shape<TPR>;
   using C = Columns<T, W, TPR, VPT, WIDE, 5>;
+  using Raw = typename C::Raw;
   constexpr int P = C::P;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float red[6][32];
-  const W *w = (const W*)a.w, *wp = (const W*)a.wp, *sv = (const W*)a.sv;
-  C col(smem, a.N);
+  const int N = (int)a.N;
+  // w and s w_post in fp32, in front of the ring
+  float *sw = reinterpret_cast<float*>(smem), *ssw = sw + (N + 3) / 4 * 4;
+  C col(smem + weight_bytes(N), N);
+  for (int j = threadIdx.x; j < N; j += S::kThreads) {
+    sw[j] = to_f<W>(((const W*)a.w)[j]);
+    ssw[j] = (a.sv ? to_f<W>(((const W*)a.sv)[j]) : a.s) * (a.wp ? to_f<W>(((const W*)a.wp)[j]) : 1.f);
+  }
+  __syncthreads();
   const int64_t step = (int64_t)gridDim.x * S::kRows, mine = threadIdx.x / TPR;
-  auto fetch = [&](int64_t base, int stage) {
-    const int64_t row = base + mine;
+  int64_t base = (int64_t)blockIdx.x * S::kRows;
+  const int64_t z = sizeof(T), r0 = base + mine;
+  const uint8_t *py = (const uint8_t*)a.y + r0 * a.y_ld * z + col.first(),
+                *pr = (const uint8_t*)a.r + r0 * a.r_ld * z + col.first(),
+                *pg = (const uint8_t*)a.gate + r0 * a.g_ld * z + col.first();
+  const int64_t sy = step * a.y_ld * z, sr = step * a.r_ld * z, sg = step * a.g_ld * z,
+                sn = step * a.N * z;
+  int64_t to = r0 * a.N * z + col.first();
+  // ahead: the row is `ahead` bytes behind the one at `to`
+  auto fetch = [&](int64_t row, int stage, int64_t ahead) {
     if (row < a.M) {
-      col.fetch(stage, 0, (const T*)a.y + row * a.y_ld);
-      col.fetch(stage, 1, (const T*)a.r + row * a.r_ld);
-      if (a.gate) col.fetch(stage, 2, (const T*)a.gate + row * a.g_ld);
-      if (a.dout) col.fetch(stage, 3, (const T*)a.dout + row * a.N);
-      if (a.dres) col.fetch(stage, 4, (const T*)a.dres + row * a.N);
+      col.fetch(stage, 0, py);
+      col.fetch(stage, 1, pr);
+      if (a.gate) col.fetch(stage, 2, pg);
+      if (a.dout) col.fetch(stage, 3, (const uint8_t*)a.dout + to + ahead);
+      if (a.dres) col.fetch(stage, 4, (const uint8_t*)a.dres + to + ahead);
     }
+    py += sy;
+    pr += sr;
+    pg += sg;
   };
-  // A vector of every input.  What is absent is filled in, so that the arithmetic has no branches:
-  // w_post with 1, a gate with 100 (its sigmoid is 1), gradients with 0.
+  // What is absent is filled in, so that the arithmetic has no branches: a gate with 100 (its
+  // sigmoid is 1), gradients with 0.
   const bool silu = a.act == FO_ACT_SILU;
   struct Part {
-    typename C::Raw y, r, z, d, dr;
-    typename C::RawW w, wp, sv;
+    Raw y, r, z, d, dr;
+    float2 w[P], sw[P];
   };
   auto load = [&](int s, int i, Part& p) {
     p.y = col.get(s, 0, i);
@@ -364,32 +414,29 @@ rrn_bwd_kernel(Bwd a) {
     p.z = a.gate ? col.get(s, 2, i) : C::template filled<T>(100.f);
     p.d = a.dout ? col.get(s, 3, i) : C::template filled<T>(0.f);
     p.dr = a.dres ? col.get(s, 4, i) : C::template filled<T>(0.f);
-    p.w = col.weights(w, i);
-    p.wp = wp ? col.weights(wp, i) : C::template filled<W>(1.f);
-    if (sv) p.sv = col.weights(sv, i);
+    col.weights(sw, i, p.w);
+    col.weights(ssw, i, p.sw);
   };
-  auto scale_of = [&](const Part& p, int q) { return sv ? C::pair(p.sv, q) : all_<float2>(a.s); };
-  float2 dw[VPT][P], ds[VPT][P], dwp[VPT][P];
+  float2 dw[VPT][P], A[VPT][P];
 #pragma unroll
   for (int i = 0; i < VPT; ++i)
 #pragma unroll
-    for (int q = 0; q < P; ++q) dw[i][q] = ds[i][q] = dwp[i][q] = all_<float2>(0.f);
-  int64_t base = (int64_t)blockIdx.x * S::kRows;
+    for (int q = 0; q < P; ++q) dw[i][q] = A[i][q] = all_<float2>(0.f);
   if constexpr (WIDE) {
-    fetch(base, 0);
+    fetch(r0, 0, 0);
     col.commit();
   }
-  for (int it = 0; base < a.M; base += step, ++it) {
+  for (int it = 0; base < a.M; base += step, to += sn, ++it) {
     const int s = it & 1;
+    const int64_t row = base + mine;
     if constexpr (WIDE) {
-      fetch(base + step, s ^ 1);
+      fetch(row + step, s ^ 1, sn);
       col.commit();
     } else {
-      fetch(base, s);
+      fetch(row, s, 0);
     }
-    const int64_t row = base + mine;
     const bool on = row < a.M;
-    const float inv1 = wp && on ? a.inv1[row] : 1.f, inv2 = on ? a.inv2[row] : 1.f;
+    const float inv1 = a.wp && on ? a.inv1[row] : 1.f, inv2 = on ? a.inv2[row] : 1.f;
     const float2 i1 = all_<float2>(inv1), i2 = all_<float2>(inv2);
     if constexpr (WIDE) col.template wait<1>();
     float2 s1 = all_<float2>(0.f), s2 = s1, s3 = s1;
@@ -401,12 +448,12 @@ rrn_bwd_kernel(Bwd a) {
 #pragma unroll
         for (int q = 0; q < P; ++q) {
           const float2 z = C::pair(p.z, q);
-          float2 av, c;
-          sigmoid_pair(z, av, c);
+          const float2 ez = map_(ex2, mul_(z, all_<float2>(-kLog2e)));
+          float2 av = map_(rcp, add_(ez, all_<float2>(1.f)));
           if (silu) av = mul_(av, z);
-          const float2 qy = mul_(mul_(scale_of(p, q), av), mul_(C::pair(p.y, q), C::pair(p.wp, q)));
+          const float2 qy = mul_(mul_(p.sw[q], av), C::pair(p.y, q));
           const float2 r2 = fma_(i1, qy, C::pair(p.r, q));
-          const float2 e = mul_(C::pair(p.d, q), C::pair(p.w, q));
+          const float2 e = mul_(C::pair(p.d, q), p.w[q]);
           s1 = fma_(e, r2, s1);
           s2 = fma_(qy, fma_(i2, e, C::pair(p.dr, q)), s2);
           s3 = fma_(qy, r2, s3);
@@ -416,41 +463,38 @@ rrn_bwd_kernel(Bwd a) {
     float sum[3] = {s1.x + s1.y, s2.x + s2.y, s3.x + s3.y};
     row_sum<TPR>(sum, red + 3 * s);
     const float c2 = inv2 * inv2 * inv2 * sum[0] / (float)a.N;
-    const float c1 = wp ? inv1 * inv1 * inv1 * fmaf(-c2, sum[2], sum[1]) / (float)a.N : 0.f;
+    const float c1 = a.wp ? inv1 * inv1 * inv1 * fmaf(-c2, sum[2], sum[1]) / (float)a.N : 0.f;
     const float2 m2 = all_<float2>(-c2), m1 = all_<float2>(-c1);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       if (on && col.on(i)) {
         Part p;
         load(s, i, p);
-        typename C::Raw dr, dy, dg;
+        Raw dr, dy, dg;
 #pragma unroll
         for (int q = 0; q < P; ++q) {
-          const float2 z = C::pair(p.z, q), wq = C::pair(p.wp, q), sj = scale_of(p, q);
-          const float2 n = mul_(C::pair(p.y, q), i1), pe = mul_(n, wq);
+          const float2 z = C::pair(p.z, q), y = C::pair(p.y, q), n = mul_(y, i1);
           float2 sg, c;
           sigmoid_pair(z, sg, c);
-          const float2 av = silu ? mul_(sg, z) : sg;
-          const float2 u = mul_(av, pe), r2 = fma_(sj, u, C::pair(p.r, q));
-          const float2 d = C::pair(p.d, q), e = mul_(d, C::pair(p.w, q));
-          const float2 D = fma_(i2, e, fma_(m2, r2, C::pair(p.dr, q))), sD = mul_(sj, D);
+          const float2 av = silu ? mul_(sg, z) : sg, sa = mul_(p.sw[q], av);
+          const float2 r2 = fma_(sa, n, C::pair(p.r, q));
+          const float2 d = C::pair(p.d, q), e = mul_(d, p.w[q]);
+          const float2 D = fma_(i2, e, fma_(m2, r2, C::pair(p.dr, q)));
           // silu' = s (1 + z c), sigmoid' = s c
           const float2 f = silu ? fma_(z, c, all_<float2>(1.f)) : c;
-          const float2 dp = mul_(sD, av);
           C::set(dr, q, D);
-          C::set(dg, q, mul_(mul_(sD, pe), mul_(sg, f)));
-          C::set(dy, q, fma_(i1, mul_(dp, wq), mul_(m1, C::pair(p.y, q))));
+          C::set(dg, q, mul_(mul_(mul_(p.sw[q], D), n), mul_(sg, f)));
+          C::set(dy, q, fma_(i1, mul_(D, sa), mul_(m1, y)));
           dw[i][q] = fma_(mul_(d, i2), r2, dw[i][q]);
-          ds[i][q] = fma_(D, u, ds[i][q]);
-          dwp[i][q] = fma_(dp, n, dwp[i][q]);
+          A[i][q] = fma_(D, mul_(av, n), A[i][q]);
         }
-        col.put((T*)a.dr + row * a.N, i, dr);
-        col.put((T*)a.dy + row * a.N, i, dy);
-        if (a.gate) col.put((T*)a.dgate + row * a.N, i, dg);
+        col.put((uint8_t*)a.dr + to, i, dr);
+        col.put((uint8_t*)a.dy + to, i, dy);
+        if (a.gate) col.put((uint8_t*)a.dgate + to, i, dg);
       }
     }
   }
-  // part[3][gridDim.x][N]; rows side by side in the CTA are added up first
+  // part[2][gridDim.x][N]; rows side by side in the CTA are added up first
   const int64_t stride = (int64_t)gridDim.x * a.N;
   float* part = a.part + (int64_t)blockIdx.x * a.N;
   if constexpr (S::kRows == 1) {
@@ -458,26 +502,22 @@ rrn_bwd_kernel(Bwd a) {
     for (int i = 0; i < VPT; ++i)
       if (col.on(i)) {
         col.put_sums(part, i, dw[i]);
-        col.put_sums(part + stride, i, ds[i]);
-        col.put_sums(part + 2 * stride, i, dwp[i]);
+        col.put_sums(part + stride, i, A[i]);
       }
   } else {
     if constexpr (WIDE) col.template wait<0>();
-    float* sums = reinterpret_cast<float*>(smem);  // [rows][3][N], over the ring
+    float* sums = reinterpret_cast<float*>(smem);  // [rows][2][N], over everything
     __syncthreads();
-    const int N = (int)a.N;
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
       if (col.on(i)) {
-        float* to = sums + mine * 3 * N;
-        col.put_sums(to, i, dw[i]);
-        col.put_sums(to + N, i, ds[i]);
-        col.put_sums(to + 2 * N, i, dwp[i]);
+        col.put_sums(sums + mine * 2 * N, i, dw[i]);
+        col.put_sums(sums + mine * 2 * N + N, i, A[i]);
       }
     __syncthreads();
-    for (int j = threadIdx.x; j < 3 * N; j += S::kThreads) {
+    for (int j = threadIdx.x; j < 2 * N; j += S::kThreads) {
       float t = 0.f;
-      for (int r = 0; r < S::kRows; ++r) t += sums[r * 3 * N + j];
+      for (int r = 0; r < S::kRows; ++r) t += sums[r * 2 * N + j];
       part[j / N * stride + j % N] = t;
     }
   }
@@ -579,7 +619,7 @@ __global__ void __launch_bounds__(256) rrn_bwd_generic_kernel(Bwd a) {
   }
 }
 
-// Partial sums of dw, ds, dw_post over a chunk of rows: a column per thread, part[3][chunks][N].
+// Partial sums of dw and A over a chunk of rows: a column per thread, part[2][chunks][N].
 template <typename T, typename W>
 __global__ void __launch_bounds__(256) rrn_cols_kernel(Bwd a) {
   const int64_t j = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -587,29 +627,26 @@ __global__ void __launch_bounds__(256) rrn_cols_kernel(Bwd a) {
   const W *wp = (const W*)a.wp, *sv = (const W*)a.sv;
   const int64_t rows = (a.M + gridDim.y - 1) / gridDim.y;
   const int64_t r0 = blockIdx.y * rows, r1 = r0 + rows < a.M ? r0 + rows : a.M;
-  const float wj = to_f<W>(((const W*)a.w)[j]), wpv = wp ? to_f<W>(wp[j]) : 1.f;
-  const float sj = sv ? to_f<W>(sv[j]) : a.s;
-  float dw = 0.f, ds = 0.f, dwp = 0.f;
+  const float wj = to_f<W>(((const W*)a.w)[j]);
+  const float sj = (sv ? to_f<W>(sv[j]) : a.s) * (wp ? to_f<W>(wp[j]) : 1.f);
+  float dw = 0.f, A = 0.f;
   for (int64_t row = r0; row < r1; ++row) {
     const float inv1 = wp ? a.inv1[row] : 1.f, inv2 = a.inv2[row];
     const float n = to_f<T>(((const T*)a.y)[row * a.y_ld + j]) * inv1;
     const float av = a.gate ? act_of(a.act, to_f<T>(((const T*)a.gate)[row * a.g_ld + j])) : 1.f;
-    const float r2 = fmaf(sj * av, n * wpv, to_f<T>(((const T*)a.r)[row * a.r_ld + j]));
+    const float r2 = fmaf(sj * av, n, to_f<T>(((const T*)a.r)[row * a.r_ld + j]));
     const float d = a.dout ? to_f<T>(((const T*)a.dout)[row * a.N + j]) : 0.f;
     const float D = fmaf(inv2, d * wj, fmaf(-a.c2[row], r2,
                          a.dres ? to_f<T>(((const T*)a.dres)[row * a.N + j]) : 0.f));
     dw = fmaf(d * r2, inv2, dw);
-    ds = fmaf(D, av * n * wpv, ds);
-    dwp = fmaf(sj * D * av, n, dwp);
+    A = fmaf(D, av * n, A);
   }
   float* part = a.part + (int64_t)blockIdx.y * a.N + j;
-  const int64_t step = (int64_t)gridDim.y * a.N;
   part[0] = dw;
-  part[step] = ds;
-  part[2 * step] = dwp;
+  part[(int64_t)gridDim.y * a.N] = A;
 }
 
-// dw, ds, dw_post from the G partial rows.  A CTA owns 32 columns; warp q adds the rows q, q + 16,
+// dw, or ds = w_post A and dw_post = s A, from the G partial rows.  A CTA owns 32 columns; warp q adds the rows q, q + 16,
 // ..., then warp 0 the 16 warps' sums: an order that does not depend on scheduling.
 constexpr int kReduceWarps = 16;
 template <typename W>
@@ -617,8 +654,7 @@ __global__ void __launch_bounds__(32 * kReduceWarps) rrn_reduce_kernel(Bwd a, in
   __shared__ float acc[kReduceWarps][33];
   const int lane = threadIdx.x & 31, q = threadIdx.x >> 5;
   const int64_t j = (int64_t)blockIdx.x * 32 + lane;
-  W* to = (W*)(blockIdx.y == 0 ? a.dw : blockIdx.y == 1 ? a.ds : a.dwp);
-  if (!to) return;
+  if (blockIdx.y == 1 && !a.ds && !a.dwp) return;
   float t = 0.f;
   if (j < a.N) {
     const float* p = a.part + blockIdx.y * (int64_t)G * a.N + j;
@@ -631,7 +667,13 @@ __global__ void __launch_bounds__(32 * kReduceWarps) rrn_reduce_kernel(Bwd a, in
     t = 0.f;
 #pragma unroll
     for (int k = 0; k < kReduceWarps; ++k) t += acc[k][lane];
-    to[j] = from_f<W>(t);
+    const W *wp = (const W*)a.wp, *sv = (const W*)a.sv;
+    if (blockIdx.y == 0) {
+      ((W*)a.dw)[j] = from_f<W>(t);
+    } else {
+      if (a.ds) ((W*)a.ds)[j] = from_f<W>(wp ? t * to_f<W>(wp[j]) : t);
+      if (a.dwp) ((W*)a.dwp)[j] = from_f<W>(t * (sv ? to_f<W>(sv[j]) : a.s));
+    }
   }
 }
 
@@ -735,8 +777,8 @@ int run_bwd(const Bwd& a, cudaStream_t st) {
   int G = 0;
   int rc = with_shape<T>(wide_ok<T>(a.N, rows, lds, 8, vs, 3), a.N, [&](auto tpr, auto vpt, auto wide) {
     using S = Shape<tpr>;
-    constexpr int ring = Columns<T, W, tpr, vpt, wide, 5>::kRingBytes;
-    const int sums = S::kRows > 1 ? (int)(S::kRows * 3 * a.N * 4) : 0;
+    const int ring = Columns<T, W, tpr, vpt, wide, 5>::kRingBytes + weight_bytes(a.N);
+    const int sums = S::kRows > 1 ? (int)(S::kRows * 2 * a.N * 4) : 0;
     const int smem = ring > sums ? ring : sums;
     int64_t ctas = num_sms() * resident(512, S::kThreads, smem);
     const int64_t need = (a.M + S::kRows - 1) / S::kRows, most = partial_rows(a.M, a.N);
@@ -753,7 +795,7 @@ int run_bwd(const Bwd& a, cudaStream_t st) {
     rc = check_launch("rrn_cols_kernel");
   }
   if (rc) return rc;
-  rrn_reduce_kernel<W><<<dim3((unsigned)((a.N + 31) / 32), 3), 32 * kReduceWarps, 0, st>>>(a, G);
+  rrn_reduce_kernel<W><<<dim3((unsigned)((a.N + 31) / 32), 2), 32 * kReduceWarps, 0, st>>>(a, G);
   return check_launch("rrn_reduce_kernel");
 }
 
@@ -811,7 +853,7 @@ extern "C" int fo_residual_rms_norm_fwd(
 extern "C" int fo_residual_rms_norm_bwd_workspace_bytes(int64_t M, int64_t N, int64_t* bytes) {
   clear_error();
   FO_CHECK_ARG(bytes && M >= 0 && N > 0, "fo_residual_rms_norm_bwd_workspace_bytes: bad argument");
-  *bytes = ((M + 3) / 4 * 4 + 3 * partial_rows(M, N) * N) * 4;  // c2 of each row, partial rows
+  *bytes = ((M + 3) / 4 * 4 + 2 * partial_rows(M, N) * N) * 4;  // c2 of each row, partial rows
   return FO_OK;
 }
 
