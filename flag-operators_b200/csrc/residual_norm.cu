@@ -145,14 +145,9 @@ struct Columns<T, W, TPR, VPT, true, S> {
       r.u[k] = ld_global_nc_v4(w + (v0 + i * TPR) * E + k * Vec16<W>::E);
     return r;
   }
-  // Of fp32 weights in shared memory
-  __device__ __forceinline__ void weights(const float* smem, int i, float2 (&f)[P]) const {
-#pragma unroll
-    for (int q = 0; q < P; q += 2) {
-      const float4 v = *reinterpret_cast<const float4*>(smem + (v0 + i * TPR) * E + 2 * q);
-      f[q] = make_float2(v.x, v.y);
-      f[q + 1] = make_float2(v.z, v.w);
-    }
+  // Pair q of fp32 weights in shared memory
+  __device__ __forceinline__ float2 weight(const float* smem, int i, int q) const {
+    return *reinterpret_cast<const float2*>(smem + (v0 + i * TPR) * E + 2 * q);
   }
   __device__ __forceinline__ void put(uint8_t* p, int i, const Raw& r) const {
     st_global_stream_v4(p + i * TPR * 16, r.u[0]);
@@ -196,8 +191,8 @@ struct Columns<T, W, TPR, VPT, false, S> {
   __device__ __forceinline__ RawW weights(const W* w, int i) const {
     return {{w[at(i, 0)], at(i, 1) < N ? w[at(i, 1)] : from_f<W>(0.f)}};
   }
-  __device__ __forceinline__ void weights(const float* smem, int i, float2 (&f)[1]) const {
-    f[0] = make_float2(smem[at(i, 0)], at(i, 1) < N ? smem[at(i, 1)] : 0.f);
+  __device__ __forceinline__ float2 weight(const float* smem, int i, int) const {
+    return make_float2(smem[at(i, 0)], at(i, 1) < N ? smem[at(i, 1)] : 0.f);
   }
   __device__ __forceinline__ void put(uint8_t* p, int i, const Raw& r) const {
     reinterpret_cast<T*>(p)[2 * i * TPR] = r.e[0];
@@ -233,6 +228,13 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float (*red)[32]) {
   }
 }
 
+// 1 / sqrt(x): the approximation (2 ulp) and one Newton step, which has to be left out where x is
+// infinite.
+__device__ __forceinline__ float inv_sqrt(float x) {
+  const float r = rsqrtf(x);
+  return x < INFINITY ? r * fmaf(-0.5f * x * r, r, 1.5f) : r;
+}
+
 // sigmoid(z) and 1 - sigmoid(z) of pairs: e = e^-z, s = 1 / (1 + e), c = e s.  e is kept below
 // 2^126, so that e s is 1 (and s 1e-38 instead of 0) at the far end.
 __device__ __forceinline__ void sigmoid_pair(float2 z, float2& s, float2& c) {
@@ -254,7 +256,7 @@ rrn_fwd_kernel(Fwd a) {
   __shared__ float red[4][32];
   const W *w = (const W*)a.w, *wp = (const W*)a.wp, *sv = (const W*)a.sv;
   C col(smem, a.N);
-  const float n = (float)a.N;
+  const float rn = 1.f / (float)a.N;
   const int64_t step = (int64_t)gridDim.x * S::kRows, mine = threadIdx.x / TPR;
   int64_t base = (int64_t)blockIdx.x * S::kRows;
   // what is fetched next, and what is written: the thread's first bytes of its row
@@ -301,7 +303,7 @@ rrn_fwd_kernel(Fwd a) {
         }
       float sum[1] = {ss.x + ss.y};
       row_sum<TPR>(sum, red + s);
-      inv1 = 1.f / sqrtf(sum[0] / n + a.eps);
+      inv1 = inv_sqrt(fmaf(sum[0], rn, a.eps));
     }
     float2 r2[VPT][P], ss = all_<float2>(0.f);
 #pragma unroll
@@ -339,7 +341,7 @@ rrn_fwd_kernel(Fwd a) {
     }
     float sum[1] = {ss.x + ss.y};
     row_sum<TPR>(sum, red + 2 + s);
-    const float inv2 = 1.f / sqrtf(sum[0] / n + a.eps);
+    const float inv2 = inv_sqrt(fmaf(sum[0], rn, a.eps));
     if (on && threadIdx.x % TPR == 0) {
       if (a.inv1) a.inv1[row] = inv1;
       if (a.inv2) a.inv2[row] = inv2;
@@ -404,9 +406,9 @@ rrn_bwd_kernel(Bwd a) {
   // What is absent is filled in, so that the arithmetic has no branches: a gate with 100 (its
   // sigmoid is 1), gradients with 0.
   const bool silu = a.act == FO_ACT_SILU;
+  const float rn = 1.f / (float)N;
   struct Part {
     Raw y, r, z, d, dr;
-    float2 w[P], sw[P];
   };
   auto load = [&](int s, int i, Part& p) {
     p.y = col.get(s, 0, i);
@@ -414,14 +416,20 @@ rrn_bwd_kernel(Bwd a) {
     p.z = a.gate ? col.get(s, 2, i) : C::template filled<T>(100.f);
     p.d = a.dout ? col.get(s, 3, i) : C::template filled<T>(0.f);
     p.dr = a.dres ? col.get(s, 4, i) : C::template filled<T>(0.f);
-    col.weights(sw, i, p.w);
-    col.weights(ssw, i, p.sw);
   };
   float2 dw[VPT][P], A[VPT][P];
 #pragma unroll
   for (int i = 0; i < VPT; ++i)
 #pragma unroll
     for (int q = 0; q < P; ++q) dw[i][q] = A[i][q] = all_<float2>(0.f);
+  float next1 = 1.f, next2 = 1.f;  // inv1 and inv2 of the row to come
+  auto invs = [&](int64_t row) {
+    if (row < a.M) {
+      if (a.wp) next1 = a.inv1[row];
+      next2 = a.inv2[row];
+    }
+  };
+  invs(r0);
   if constexpr (WIDE) {
     fetch(r0, 0, 0);
     col.commit();
@@ -436,7 +444,8 @@ rrn_bwd_kernel(Bwd a) {
       fetch(row, s, 0);
     }
     const bool on = row < a.M;
-    const float inv1 = a.wp && on ? a.inv1[row] : 1.f, inv2 = on ? a.inv2[row] : 1.f;
+    const float inv1 = next1, inv2 = next2;
+    invs(row + step);
     const float2 i1 = all_<float2>(inv1), i2 = all_<float2>(inv2);
     if constexpr (WIDE) col.template wait<1>();
     float2 s1 = all_<float2>(0.f), s2 = s1, s3 = s1;
@@ -451,9 +460,9 @@ rrn_bwd_kernel(Bwd a) {
           const float2 ez = map_(ex2, mul_(z, all_<float2>(-kLog2e)));
           float2 av = map_(rcp, add_(ez, all_<float2>(1.f)));
           if (silu) av = mul_(av, z);
-          const float2 qy = mul_(mul_(p.sw[q], av), C::pair(p.y, q));
+          const float2 qy = mul_(mul_(col.weight(ssw, i, q), av), C::pair(p.y, q));
           const float2 r2 = fma_(i1, qy, C::pair(p.r, q));
-          const float2 e = mul_(C::pair(p.d, q), p.w[q]);
+          const float2 e = mul_(C::pair(p.d, q), col.weight(sw, i, q));
           s1 = fma_(e, r2, s1);
           s2 = fma_(qy, fma_(i2, e, C::pair(p.dr, q)), s2);
           s3 = fma_(qy, r2, s3);
@@ -462,8 +471,8 @@ rrn_bwd_kernel(Bwd a) {
     }
     float sum[3] = {s1.x + s1.y, s2.x + s2.y, s3.x + s3.y};
     row_sum<TPR>(sum, red + 3 * s);
-    const float c2 = inv2 * inv2 * inv2 * sum[0] / (float)a.N;
-    const float c1 = a.wp ? inv1 * inv1 * inv1 * fmaf(-c2, sum[2], sum[1]) / (float)a.N : 0.f;
+    const float c2 = inv2 * inv2 * inv2 * (sum[0] * rn);
+    const float c1 = a.wp ? inv1 * inv1 * inv1 * (fmaf(-c2, sum[2], sum[1]) * rn) : 0.f;
     const float2 m2 = all_<float2>(-c2), m1 = all_<float2>(-c1);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -476,14 +485,15 @@ rrn_bwd_kernel(Bwd a) {
           const float2 z = C::pair(p.z, q), y = C::pair(p.y, q), n = mul_(y, i1);
           float2 sg, c;
           sigmoid_pair(z, sg, c);
-          const float2 av = silu ? mul_(sg, z) : sg, sa = mul_(p.sw[q], av);
+          const float2 wq = col.weight(ssw, i, q);
+          const float2 av = silu ? mul_(sg, z) : sg, sa = mul_(wq, av);
           const float2 r2 = fma_(sa, n, C::pair(p.r, q));
-          const float2 d = C::pair(p.d, q), e = mul_(d, p.w[q]);
+          const float2 d = C::pair(p.d, q), e = mul_(d, col.weight(sw, i, q));
           const float2 D = fma_(i2, e, fma_(m2, r2, C::pair(p.dr, q)));
           // silu' = s (1 + z c), sigmoid' = s c
           const float2 f = silu ? fma_(z, c, all_<float2>(1.f)) : c;
           C::set(dr, q, D);
-          C::set(dg, q, mul_(mul_(mul_(p.sw[q], D), n), mul_(sg, f)));
+          C::set(dg, q, mul_(mul_(mul_(wq, D), n), mul_(sg, f)));
           C::set(dy, q, fma_(i1, mul_(D, sa), mul_(m1, y)));
           dw[i][q] = fma_(mul_(d, i2), r2, dw[i][q]);
           A[i][q] = fma_(D, mul_(av, n), A[i][q]);
@@ -712,9 +722,10 @@ template <typename T, typename F> int with_shape(bool wide, int64_t N, F&& f) {
     FO_SHAPE(512, 2, E, std::true_type);
   } else {
     FO_SHAPE(32, 1, 2, std::false_type);
-    FO_SHAPE(32, 4, 2, std::false_type);
-    FO_SHAPE(128, 4, 2, std::false_type);
-    FO_SHAPE(256, 4, 2, std::false_type);
+    FO_SHAPE(32, 2, 2, std::false_type);
+    FO_SHAPE(128, 2, 2, std::false_type);
+    FO_SHAPE(256, 2, 2, std::false_type);
+    FO_SHAPE(512, 2, 2, std::false_type);
     FO_SHAPE(512, 4, 2, std::false_type);
   }
 #undef FO_SHAPE
