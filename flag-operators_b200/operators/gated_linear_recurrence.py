@@ -70,7 +70,7 @@ def _strides(*ts):
 
 def _forward(x, g, beta, decay, h0, reset, scale, want_state, want_ckpt):
     B, L, C = x.shape
-    h = torch.empty((B, L, C), dtype=x.dtype, device=x.device)
+    h = x.new_empty((B, L, C))
     hT = torch.empty((B, C), dtype=torch.float32, device=x.device) if want_state else None
     ckpt = torch.empty((B, -(-L // CHECKPOINT), C), dtype=torch.float32, device=x.device) \
         if want_ckpt else None
@@ -89,9 +89,7 @@ def _backward(x, g, beta, decay, reset, ckpt, scale, dh, dhT, need_dh0, need_dde
         else dh.to(x.dtype).contiguous()
     if dhT is not None:
         dhT = dhT.to(torch.float32).contiguous()
-    dx = torch.empty((B, L, C), dtype=x.dtype, device=dev)
-    dg = torch.empty((B, L, C), dtype=g.dtype, device=dev)
-    dbeta = torch.empty((B, L, C), dtype=g.dtype, device=dev)
+    dx, dg, dbeta = x.new_empty((B, L, C)), g.new_empty((B, L, C)), g.new_empty((B, L, C))
     dh0 = torch.empty((B, C), dtype=torch.float32, device=dev) if need_dh0 else None
     ddecay = torch.empty(C, dtype=torch.float32, device=dev) if need_ddecay else None
     ws, nbytes = None, ctypes.c_int64(0)
@@ -199,7 +197,7 @@ def gated_linear_recurrence_step(
         decay = decay.to(torch.float32).contiguous()
     x, g, beta = _rows(x), _rows(g), _rows(beta)
     B, C = x.shape
-    h = torch.empty((B, C), dtype=x.dtype, device=x.device)
+    h = x.new_empty((B, C))
     with _lib.on_device(x):
         _lib.call("fo_glr_step", _lib.ptr(x), _lib.ptr(g), _lib.ptr(beta), _lib.ptr(decay),
                   _lib.ptr(state), _lib.ptr(h), B, C, _strides(x, g, beta), float(decay_scale),

@@ -50,6 +50,13 @@ def _rows(t, N):
     return (t, ld) if ok else (t.contiguous(), N)
 
 
+def _inv_ptrs(inv, M):
+    if inv is None:
+        return None, None
+    p = inv.data_ptr()
+    return ctypes.c_void_p(p), ctypes.c_void_p(p + 4 * M)
+
+
 def _forward(y, residual, weight, post_weight, gate, act, scale, eps, keep):
     N = weight.numel()
     M = y.numel() // N
@@ -57,26 +64,23 @@ def _forward(y, residual, weight, post_weight, gate, act, scale, eps, keep):
     residual, r_ld = _rows(residual, N)
     gate, g_ld = _rows(gate, N) if gate is not None else (None, 0)
     dev = y.device
-    out = torch.empty(y.shape, dtype=y.dtype, device=dev)
-    res = torch.empty(y.shape, dtype=y.dtype, device=dev)
-    inv1 = torch.empty(M, dtype=torch.float32, device=dev) \
-        if keep and post_weight is not None else None
-    inv2 = torch.empty(M, dtype=torch.float32, device=dev) if keep else None
+    out, res = y.new_empty(y.shape), y.new_empty(y.shape)
+    inv = torch.empty(2 * M, dtype=torch.float32, device=dev) if keep else None  # inv1, inv2
     sv, s = (scale, 1.0) if isinstance(scale, torch.Tensor) else (None, scale)
     with _lib.on_device(y):
         _lib.call("fo_residual_rms_norm_fwd", _lib.ptr(y), _lib.ptr(residual), _lib.ptr(weight),
                   _lib.ptr(post_weight), _lib.ptr(gate), _lib.ptr(sv), s, _lib.ptr(out),
-                  _lib.ptr(res), _lib.ptr(inv1), _lib.ptr(inv2), M, N, y_ld, r_ld, g_ld, eps, act,
+                  _lib.ptr(res), *_inv_ptrs(inv, M), M, N, y_ld, r_ld, g_ld, eps, act,
                   _lib.dtype_code(y.dtype), _lib.dtype_code(weight.dtype), _lib.stream_of(y))
-    return out, res, inv1, inv2
+    return out, res, inv
 
 
 class _ResidualRmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, residual, weight, post_weight, gate, scale, act, eps):
-        out, res, inv1, inv2 = _forward(y, residual, weight, post_weight, gate, act, scale, eps, True)
+        out, res, inv = _forward(y, residual, weight, post_weight, gate, act, scale, eps, True)
         sv = scale if isinstance(scale, torch.Tensor) else None
-        ctx.save_for_backward(y, residual, weight, post_weight, gate, sv, inv1, inv2)
+        ctx.save_for_backward(y, residual, weight, post_weight, gate, sv, inv)
         ctx.s = 1.0 if sv is not None else scale
         ctx.act = act
         ctx.set_materialize_grads(False)
@@ -85,7 +89,7 @@ class _ResidualRmsNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, dres):
-        y, residual, weight, post_weight, gate, sv, inv1, inv2 = ctx.saved_tensors
+        y, residual, weight, post_weight, gate, sv, inv = ctx.saved_tensors
         if dout is None and dres is None:
             return (None,) * 8
         N = weight.numel()
@@ -96,9 +100,8 @@ class _ResidualRmsNorm(torch.autograd.Function):
         dev = y.device
         dout = None if dout is None else dout.to(y.dtype).contiguous()
         dres = None if dres is None else dres.to(y.dtype).contiguous()
-        dy = torch.empty(y.shape, dtype=y.dtype, device=dev)
-        dr = torch.empty(y.shape, dtype=y.dtype, device=dev)
-        dgate = torch.empty(y.shape, dtype=y.dtype, device=dev) if gate is not None else None
+        dy, dr = y.new_empty(y.shape), y.new_empty(y.shape)
+        dgate = y.new_empty(y.shape) if gate is not None else None
         dw = torch.empty_like(weight)
         dwp = torch.empty_like(post_weight) if post_weight is not None else None
         ds = torch.empty_like(sv) if sv is not None else None
@@ -108,8 +111,8 @@ class _ResidualRmsNorm(torch.autograd.Function):
             ws = torch.empty(max(nbytes.value, 1), dtype=torch.uint8, device=dev)
             _lib.call("fo_residual_rms_norm_bwd", _lib.ptr(dout), _lib.ptr(dres), _lib.ptr(y),
                       _lib.ptr(residual), _lib.ptr(weight), _lib.ptr(post_weight), _lib.ptr(gate),
-                      _lib.ptr(sv), ctx.s, _lib.ptr(inv1), _lib.ptr(inv2), _lib.ptr(dy),
-                      _lib.ptr(dr), _lib.ptr(dgate), _lib.ptr(dw), _lib.ptr(dwp), _lib.ptr(ds),
+                      _lib.ptr(sv), ctx.s, *_inv_ptrs(inv, M), _lib.ptr(dy), _lib.ptr(dr),
+                      _lib.ptr(dgate), _lib.ptr(dw), _lib.ptr(dwp), _lib.ptr(ds),
                       M, N, y_ld, r_ld, g_ld, ctx.act, _lib.dtype_code(y.dtype),
                       _lib.dtype_code(weight.dtype), _lib.ptr(ws), nbytes.value, _lib.stream_of(y))
         need = ctx.needs_input_grad
@@ -175,5 +178,5 @@ def residual_rms_norm(
             isinstance(t, torch.Tensor) and t.requires_grad
             for t in (y, residual, weight, post_weight, gate, scale)):
         return _ResidualRmsNorm.apply(y, residual, weight, post_weight, gate, scale, act, float(eps))
-    out, res, _, _ = _forward(y, residual, weight, post_weight, gate, act, scale, float(eps), False)
+    out, res, _ = _forward(y, residual, weight, post_weight, gate, act, scale, float(eps), False)
     return out, res

@@ -53,7 +53,7 @@ def _padding(op, padding_idx, V):
 
 def _forward(ids, weight, scale):
     V, N = weight.shape
-    out = torch.empty((*ids.shape, N), dtype=weight.dtype, device=weight.device)
+    out = weight.new_empty((*ids.shape, N))
     with _lib.on_device(weight):
         _lib.call("fo_embedding_fwd", _lib.ptr(ids), _lib.ptr(weight), _lib.ptr(out), ids.numel(),
                   V, N, weight.stride(0) if V > 1 else N, scale, _lib.dtype_code(weight.dtype),
@@ -64,7 +64,7 @@ def _forward(ids, weight, scale):
 def _backward(dout, ids, V, scale, padding_idx):
     N, T = dout.shape[-1], ids.numel()
     dout = dout.contiguous()
-    dw = torch.empty((V, N), dtype=dout.dtype, device=dout.device)
+    dw = dout.new_empty((V, N))
     nbytes = ctypes.c_int64(0)
     with _lib.on_device(dout):
         _lib.call("fo_embedding_bwd_workspace_bytes", T, V, N, ctypes.byref(nbytes))

@@ -401,7 +401,7 @@ FO_API int fo_gdr_bwd(const void* q, const void* k, const void* v, const void* b
  * h: [B, L, C] contiguous, dtype.  gate_dtype is dtype or FO_F32.
  * strides: batch and step strides of x, g, beta in elements (six numbers); channels are
  * contiguous.  ckpt, for the backward: [B, ceil(L / FO_GLR_CHECKPOINT), C] fp32 or NULL, the
- * state in front of every FO_GLR_CHECKPOINT-th step.  B <= 65535.
+ * state in front of every FO_GLR_CHECKPOINT-th step.
  */
 #define FO_GLR_CHECKPOINT 64
 FO_API int fo_glr_fwd(const void* x, const void* g, const void* beta, const float* decay,

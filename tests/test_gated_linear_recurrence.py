@@ -501,8 +501,8 @@ def test_c_entry_checks():
     nul = [None] * 9
     with pytest.raises(ValueError, match="negative size"):
         _lib.call("fo_glr_fwd", *nul, -1, 4, 4, None, 1.0, f32, f32, None)
-    with pytest.raises(ValueError, match="over 65535"):
-        _lib.call("fo_glr_fwd", *nul, 65536, 4, 4, None, 1.0, f32, f32, None)
+    with pytest.raises(ValueError, match="over the grid's limit"):
+        _lib.call("fo_glr_fwd", *nul, 1 << 31, 4, 4, None, 1.0, f32, f32, None)
     with pytest.raises(ValueError, match="null pointer"):
         _lib.call("fo_glr_fwd", *nul, 1, 4, 4, None, 1.0, f32, f32, None)
     st = _lib.i64_array([0] * 6)
