@@ -34,12 +34,17 @@
 namespace fo {
 namespace {
 
-constexpr int kSteps = 8;                  // steps of a thread in a tile
-constexpr int kWarps = 8;                  // warps of a CTA, along time
-constexpr int kTile = kSteps * kWarps;     // steps of a CTA in a round
+constexpr int kFwdSteps = 16, kFwdWarps = 8;  // steps of a thread in a round, and warps of a CTA
+constexpr int kFwdTile = kFwdSteps * kFwdWarps;
+constexpr int kBwdSteps = 8, kBwdWarps = 8;
+constexpr int kBwdTile = kBwdSteps * kBwdWarps;
+constexpr int kBwdCluster = 4;                // CTAs of a cluster, at most
+constexpr int kFwdCluster = 8;
+constexpr int kFwdWant = 1, kBwdWant = 1;     // CTAs an SM below which clusters are made
 constexpr int kStages = 2;                 // tiles of the ring
-constexpr int kThreads = 32 * kWarps;
-static_assert(kTile == FO_GLR_CHECKPOINT, "a tile begins at a checkpoint");
+static_assert(kBwdTile == FO_GLR_CHECKPOINT, "a tile of the backward begins at a checkpoint");
+static_assert(kFwdCluster <= kFwdWarps && kBwdCluster <= kBwdWarps, "a warp for each CTA");
+static_assert(FO_GLR_CHECKPOINT % kFwdSteps == 0, "a warp's steps begin at a checkpoint or have none");
 
 struct Strides {
   int64_t xb, xl, gb, gl, bb, bl;  // batch and step strides of x, g, beta, in elements
@@ -118,33 +123,50 @@ template <typename T, int V> struct Elem {
     }
   }
 };
-// A warp's kSteps rows of a stream into its part of the ring; lanes without a channel and rows from
-// `rows` on are left out.  wide: 16 bytes a copy, rows shared out over the lanes (so a __syncwarp
-// has to follow the wait); otherwise every lane copies just its own elements.
-template <typename T, int V>
-__device__ __forceinline__ void copy_rows(uint8_t (*ring)[32 * Elem<T, V>::kBytes], const T* row0,
-                                          int64_t step, int64_t C_left, int rows, bool wide) {
+// One input of a warp: STEPS rows a round into its part of the ring, `round` bytes apart in memory
+// from one round to the next.  wide: 16 bytes a copy, rows shared out over the lanes (so a
+// __syncwarp has to follow the wait); otherwise every lane copies just its own elements.  Lanes
+// without a channel and rows from `rows` on are left out.
+template <typename T, int V, int STEPS> struct Stream {
   using E = Elem<T, V>;
-  const int lane = threadIdx.x & 31;
-  if (wide) {
-    constexpr int kPer = 16 / (int)sizeof(T);         // elements of a copy
-    constexpr int kRow = 32 * V / kPer;               // copies of a row
-#pragma unroll
-    for (int k = 0; k < (kSteps * kRow) / 32; ++k) {
-      const int r = (k * 32 + lane) / kRow, c = (lane % kRow) * kPer;
-      if (r < rows && c < C_left)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                         (uint32_t)__cvta_generic_to_shared(&ring[r][c * (int)sizeof(T)])),
-                     "l"(row0 + r * step + c)
-                     : "memory");
-    }
-  } else if (lane * V < C_left) {
-    const T* p = row0 + lane * V;
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i, p += step)
-      if (i < rows) E::copy(&ring[i][lane * E::kBytes], p);
+  static constexpr int kRow = 32 * E::kBytes;     // bytes of a row in the ring
+  static constexpr int kBytes = STEPS * kRow;     // of a warp's part of a stage
+  static constexpr int kPer = 512 / kRow;         // rows of a warp's 16-byte copies
+  const uint8_t* p;
+  int64_t step, round;
+  int row0;
+  bool on, wide;
+  // first: the first element of the slab in the warp's first row; left: channels of the slab
+  __device__ __forceinline__ Stream(const T* first, int64_t step_, int64_t round_, int64_t left,
+                                    bool wide_)
+      : step(step_ * (int)sizeof(T)), round(round_ * (int)sizeof(T)), wide(wide_) {
+    const int lane = threadIdx.x & 31;
+    row0 = wide ? lane / (kRow / 16) : 0;
+    const int byte = wide ? lane % (kRow / 16) * 16 : lane * E::kBytes;
+    on = byte < left * (int)sizeof(T);
+    p = reinterpret_cast<const uint8_t*>(first) + row0 * step + byte;
   }
-}
+  __device__ __forceinline__ void fetch(uint8_t* ring, int rows) {
+    const int lane = threadIdx.x & 31;
+    if (on) {
+      if (wide) {
+        const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
+        const uint8_t* q = p;
+#pragma unroll
+        for (int k = 0; k < STEPS / kPer; ++k, q += kPer * step)
+          if (rows == STEPS || k * kPer + row0 < rows)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + k * 512), "l"(q)
+                         : "memory");
+      } else {
+        const uint8_t* q = p;
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i, q += step)
+          if (i < rows) E::copy(ring + i * kRow + lane * E::kBytes, reinterpret_cast<const T*>(q));
+      }
+    }
+    p += round;
+  }
+};
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
@@ -184,27 +206,25 @@ __device__ __forceinline__ void store_remote(void* smem, uint32_t cta, float2 v)
 
 // The maps of a round: of the CTA's warps, and (clusters) of the cluster's CTAs.  Two copies,
 // used in turn: a copy is written again only after a barrier that every reader of it has passed.
-template <typename F, bool CLUSTER> struct Maps {
-  F A[2][kWarps][32], H[2][kWarps][32];
-  F cA[2][CLUSTER ? 8 : 1][32], cH[2][CLUSTER ? 8 : 1][32];
+template <typename F, int WARPS, int CTAS> struct Maps {
+  F A[2][WARPS][32], H[2][WARPS][32];
+  F cA[2][CTAS][32], cH[2][CTAS][32];
 };
 
-// From this warp's map (A, H) and the state S in front of the round: the state in front of
-// this warp's steps; S becomes the state behind the round.  REVERSE walks the warps and CTAs from
-// the last to the first.  entering: the state in front of the CTA's tile.
-template <typename F, bool CLUSTER, bool REVERSE, bool RESET>
-__device__ __forceinline__ F carry_in(Maps<F, CLUSTER>& m, int parity, F A, F H, F& S, F& entering) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  m.A[parity][w][lane] = finite(A);
-  m.H[parity][w][lane] = H;
-  __syncthreads();
-  if constexpr (CLUSTER) {
+// With the maps of all warps in place, and the state S in front of the round: the state in front of
+// warp w's steps; S becomes the state behind the round.  REVERSE walks the warps and CTAs from the
+// last to the first.
+template <bool REVERSE, bool RESET, typename F, int WARPS, int CTAS>
+__device__ __forceinline__ F carry_in(Maps<F, WARPS, CTAS>& m, int parity, int w, F& S) {
+  const int lane = threadIdx.x & 31;
+  F mine = S;
+  if constexpr (CTAS > 1) {
     const uint32_t n = cluster_size(), me = cluster_rank();
     if (w < (int)n) {  // warp w hands the CTA's map to CTA w
       F a = all_<F>(1.f), h = all_<F>(0.f);
 #pragma unroll
-      for (int k = 0; k < kWarps; ++k) {
-        const int q = REVERSE ? kWarps - 1 - k : k;
+      for (int k = 0; k < WARPS; ++k) {
+        const int q = REVERSE ? WARPS - 1 - k : k;
         const F ak = m.A[parity][q][lane];
         h = through<RESET>(h, ak, m.H[parity][q][lane]);
         a = finite(mul_(a, ak));
@@ -213,31 +233,25 @@ __device__ __forceinline__ F carry_in(Maps<F, CLUSTER>& m, int parity, F A, F H,
       store_remote(&m.cH[parity][me][lane], w, h);
     }
     cluster_barrier();
-    F mine = S;
     for (uint32_t k = 0; k < n; ++k) {
       const uint32_t q = REVERSE ? n - 1 - k : k;
       if (q == me) mine = S;
       S = through<RESET>(S, m.cA[parity][q][lane], m.cH[parity][q][lane]);
     }
-    entering = mine;
-    F s = mine;
 #pragma unroll
-    for (int k = 0; k < kWarps - 1; ++k) {
-      const int q = REVERSE ? kWarps - 1 - k : k;
-      if (REVERSE ? q > w : q < w) s = through<RESET>(s, m.A[parity][q][lane], m.H[parity][q][lane]);
+    for (int k = 0; k < WARPS - 1; ++k) {
+      const int q = REVERSE ? WARPS - 1 - k : k;
+      if (REVERSE ? q > w : q < w) mine = through<RESET>(mine, m.A[parity][q][lane], m.H[parity][q][lane]);
     }
-    return s;
   } else {
-    entering = S;
-    F mine = S;
 #pragma unroll 4  // more would hold the maps of all warps in registers at once
-    for (int k = 0; k < kWarps; ++k) {
-      const int q = REVERSE ? kWarps - 1 - k : k;
+    for (int k = 0; k < WARPS; ++k) {
+      const int q = REVERSE ? WARPS - 1 - k : k;
       if (q == w) mine = S;
       S = through<RESET>(S, m.A[parity][q][lane], m.H[parity][q][lane]);
     }
-    return mine;
   }
+  return mine;
 }
 
 // What a thread's place is: batch b, first channel c, rank and size of the cluster.
@@ -258,10 +272,15 @@ template <int V, bool CLUSTER> __device__ __forceinline__ Place place(int64_t C)
   return p;
 }
 
-// Bit i: the warp's step t0 + i is a reset (steps from L on are not).
-__device__ __forceinline__ uint32_t reset_bits(const uint8_t* reset, int64_t t0, int64_t L) {
+// The warp of the thread, in a form that the compiler knows to be the same for all lanes.
+__device__ __forceinline__ int warp_index() {
+  return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
+}
+
+// Bit i: the warp's step t0 + i is a reset (of its `rows` steps).
+__device__ __forceinline__ uint32_t reset_bits(const uint8_t* reset, int64_t t0, int rows) {
   const int lane = threadIdx.x & 31;
-  const bool r = lane < kSteps && t0 + lane < L && reset[t0 + lane] != 0;
+  const bool r = lane < rows && reset[t0 + lane] != 0;
   return __ballot_sync(0xffffffffu, r);
 }
 
@@ -269,13 +288,13 @@ __device__ __forceinline__ uint32_t reset_bits(const uint8_t* reset, int64_t t0,
 // Forward
 // ---------------------------------------------------------------------------
 template <typename T, typename G, int V> struct FwdRing {
-  uint8_t x[kStages][kWarps][kSteps][32 * Elem<T, V>::kBytes];
-  uint8_t g[kStages][kWarps][kSteps][32 * Elem<G, V>::kBytes];
-  uint8_t b[kStages][kWarps][kSteps][32 * Elem<G, V>::kBytes];
+  uint8_t x[kStages][kFwdWarps][Stream<T, V, kFwdSteps>::kBytes];
+  uint8_t g[kStages][kFwdWarps][Stream<G, V, kFwdSteps>::kBytes];
+  uint8_t b[kStages][kFwdWarps][Stream<G, V, kFwdSteps>::kBytes];
 };
 
 template <typename T, typename G, int V, bool LOGITS, bool RESET, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(32 * kFwdWarps, 2)
 glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __restrict__ beta,
                const float* __restrict__ decay, const float* __restrict__ h0,
                const uint8_t* __restrict__ reset, T* __restrict__ h, float* __restrict__ hT,
@@ -283,15 +302,19 @@ glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
   using F = typename Lane<V>::F;
   using EX = Elem<T, V>;
   using EG = Elem<G, V>;
+  constexpr int N = kFwdSteps;
   extern __shared__ __align__(16) uint8_t smem[];
   auto& ring = *reinterpret_cast<FwdRing<T, G, V>*>(smem);
-  __shared__ Maps<F, CLUSTER> maps;
+  __shared__ Maps<F, kFwdWarps, CLUSTER ? kFwdCluster : 1> maps;
   const Place p = place<V, CLUSTER>(C);
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int64_t tiles = (L + kTile - 1) / kTile, rounds = (tiles + p.size - 1) / p.size;
-  x += p.b * st.xb + p.c0;
-  g += p.b * st.gb + p.c0;
-  beta += p.b * st.bb + p.c0;
+  const int lane = threadIdx.x & 31, w = warp_index();
+  const int64_t tiles = (L + kFwdTile - 1) / kFwdTile, rounds = (tiles + p.size - 1) / p.size;
+  const int64_t checkpoints = (L + FO_GLR_CHECKPOINT - 1) / FO_GLR_CHECKPOINT;
+  const int64_t per_round = (int64_t)p.size * kFwdTile;
+  int64_t t0 = (int64_t)p.rank * kFwdTile + w * N;  // the warp's first step of the round
+  Stream<T, V, N> in_x(x + p.b * st.xb + t0 * st.xl + p.c0, st.xl, per_round * st.xl, C - p.c0, wide);
+  Stream<G, V, N> in_g(g + p.b * st.gb + t0 * st.gl + p.c0, st.gl, per_round * st.gl, C - p.c0, wide);
+  Stream<G, V, N> in_b(beta + p.b * st.bb + t0 * st.bl + p.c0, st.bl, per_round * st.bl, C - p.c0, wide);
   if (RESET) reset += p.b * L;
   F r1 = all_<F>(0.f), r2 = all_<F>(0.f);  // log2 a and -2 log a of an open gate
   F S = all_<F>(0.f);
@@ -304,32 +327,32 @@ glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
     }
     if (h0) S = Elem<float, V>::load(h0 + p.b * C + p.c);
   }
-  auto rows_of = [&](int64_t t0) { return t0 < L ? (int)(L - t0 < kSteps ? L - t0 : kSteps) : 0; };
-  auto fetch = [&](int64_t round) {
-    const int64_t t0 = (round * p.size + p.rank) * kTile + w * kSteps;
-    const int s = (int)(round % kStages), n = rows_of(t0);
-    if (n > 0) {
-      copy_rows<T, V>(ring.x[s][w], x + t0 * st.xl, st.xl, C - p.c0, n, wide);
-      copy_rows<G, V>(ring.g[s][w], g + t0 * st.gl, st.gl, C - p.c0, n, wide);
-      copy_rows<G, V>(ring.b[s][w], beta + t0 * st.bl, st.bl, C - p.c0, n, wide);
+  auto rows_of = [&](int64_t t) { return t < L ? (int)(L - t < N ? L - t : N) : 0; };
+  int64_t t_fetch = t0;
+  auto fetch = [&](int stage) {
+    if (const int n = rows_of(t_fetch)) {
+      in_x.fetch(ring.x[stage][w], n);
+      in_g.fetch(ring.g[stage][w], n);
+      in_b.fetch(ring.b[stage][w], n);
     }
+    t_fetch += per_round;
     copy_commit();
   };
 #pragma unroll
   for (int k = 0; k < kStages - 1; ++k) fetch(k);
-  for (int64_t round = 0; round < rounds; ++round) {
-    const int64_t tile = round * p.size + p.rank, t0 = tile * kTile + w * kSteps;
+  T* to = h + (p.b * L + t0) * C + p.c0;
+  for (int64_t round = 0; round < rounds; ++round, t0 += per_round, to += per_round * C) {
     const int n = rows_of(t0), s = (int)(round % kStages);
-    fetch(round + kStages - 1);
-    const uint32_t rs = RESET ? reset_bits(reset, t0, L) : 0;
+    fetch((int)((round + kStages - 1) % kStages));
+    const uint32_t rs = RESET ? reset_bits(reset, t0, n) : 0;
     copy_wait<kStages - 1>();
     __syncwarp();
-    F a[kSteps], b[kSteps], A = all_<F>(1.f), H = all_<F>(0.f);
+    F a[N], b[N], A = all_<F>(1.f), H = all_<F>(0.f);
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      const F xv = EX::load(&ring.x[s][w][i][lane * EX::kBytes]);
-      const F gv = EG::load(&ring.g[s][w][i][lane * EG::kBytes]);
-      const F bv = EG::load(&ring.b[s][w][i][lane * EG::kBytes]);
+    for (int i = 0; i < N; ++i) {
+      const F xv = EX::load(&ring.x[s][w][(i * 32 + lane) * EX::kBytes]);
+      const F gv = EG::load(&ring.g[s][w][(i * 32 + lane) * EG::kBytes]);
+      const F bv = EG::load(&ring.b[s][w][(i * 32 + lane) * EG::kBytes]);
       if (LOGITS) {
         // 1 / (1 + e^-z): 0 and 1 at -inf and +inf
         auto sig = [](F z) {
@@ -347,35 +370,38 @@ glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
       }
       if (RESET && (rs >> i & 1)) a[i] = all_<F>(0.f);
     }
-    if (n < kSteps) {  // behind the end: the state passes
+    if (n < N) {  // behind the end: the state passes
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i)
+      for (int i = 0; i < N; ++i)
         if (i >= n) {
           a[i] = all_<F>(1.f);
           b[i] = all_<F>(0.f);
         }
     }
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
+    for (int i = 0; i < N; ++i) {
       if (RESET && (rs >> i & 1)) H = all_<F>(0.f);
       A = mul_(A, a[i]);
       H = fma_(a[i], H, b[i]);
     }
-    F entering;
-    F hv = carry_in<F, CLUSTER, false, RESET>(maps, (int)(round & 1), A, H, S, entering);
+    const int parity = (int)(round & 1);
+    maps.A[parity][w][lane] = finite(A);
+    maps.H[parity][w][lane] = H;
+    __syncthreads();
+    F hv = carry_in<false, RESET>(maps, parity, w, S);
     if (p.on) {
-      if (ckpt && w == 0 && tile < tiles)
-        Elem<float, V>::store(ckpt + (p.b * tiles + tile) * C + p.c, entering);
-      T* hp = h + (p.b * L + t0) * C + p.c;
+      if (ckpt && n > 0 && t0 % FO_GLR_CHECKPOINT == 0)
+        Elem<float, V>::store(ckpt + (p.b * checkpoints + t0 / FO_GLR_CHECKPOINT) * C + p.c, hv);
       auto walk = [&](auto full) {
+        T* q = to;
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i, hp += C) {
+        for (int i = 0; i < N; ++i, q += C) {
           if (RESET && (rs >> i & 1)) hv = all_<F>(0.f);
           hv = fma_(a[i], hv, b[i]);
-          if (full || i < n) EX::store(hp, hv);
+          if (full || i < n) EX::store(q + lane * V, hv);
         }
       };
-      if (n == kSteps) walk(std::true_type{});
+      if (n == N) walk(std::true_type{});
       else walk(std::false_type{});
       // the warp that has the last step
       if (hT && n > 0 && t0 + n == L) Elem<float, V>::store(hT + p.b * C + p.c, hv);
@@ -390,33 +416,50 @@ glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
 // Backward
 // ---------------------------------------------------------------------------
 template <typename T, typename G, int V> struct BwdRing {
-  FwdRing<T, G, V> in;
-  uint8_t d[kStages][kWarps][kSteps][32 * Elem<T, V>::kBytes];
-  // lo_b of the round between its first and last walk: in registers it would spill
-  typename Lane<V>::F lo_b[kWarps][kSteps][32];
+  using F = typename Lane<V>::F;
+  uint8_t x[kStages][kBwdWarps][Stream<T, V, kBwdSteps>::kBytes];
+  uint8_t d[kStages][kBwdWarps][Stream<T, V, kBwdSteps>::kBytes];
+  uint8_t g[kStages][kBwdWarps][Stream<G, V, kBwdSteps>::kBytes];
+  uint8_t b[kStages][kBwdWarps][Stream<G, V, kBwdSteps>::kBytes];
+  // Of the round between its first and last walk, where registers would spill: m i and
+  // a^2 / (1 - a^2); 1 - i takes the place of g and beta in the ring.
+  F mi[kBwdWarps][kBwdSteps][32], q[kBwdWarps][kBwdSteps][32];
+
+  // one F a lane in the places of g and beta of step i, which are not needed any more
+  __device__ __forceinline__ void put_gates(int s, int w, int i, int lane, F f) {
+    uint8_t *pg = &g[s][w][(i * 32 + lane) * Elem<G, V>::kBytes],
+            *pb = &b[s][w][(i * 32 + lane) * Elem<G, V>::kBytes];
+    if constexpr (V == 2) {
+      *reinterpret_cast<float*>(pg) = f.x;
+      *reinterpret_cast<float*>(pb) = f.y;
+    } else if constexpr (sizeof(G) == 4) {
+      *reinterpret_cast<float*>(pg) = f;
+    } else {
+      *reinterpret_cast<uint16_t*>(pg) = (uint16_t)(__float_as_uint(f) >> 16);
+      *reinterpret_cast<uint16_t*>(pb) = (uint16_t)__float_as_uint(f);
+    }
+  }
+  __device__ __forceinline__ F get_gates(int s, int w, int i, int lane) const {
+    const uint8_t *pg = &g[s][w][(i * 32 + lane) * Elem<G, V>::kBytes],
+                  *pb = &b[s][w][(i * 32 + lane) * Elem<G, V>::kBytes];
+    if constexpr (V == 2)
+      return make_float2(*reinterpret_cast<const float*>(pg), *reinterpret_cast<const float*>(pb));
+    else if constexpr (sizeof(G) == 4)
+      return *reinterpret_cast<const float*>(pg);
+    else
+      return __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(pg) << 16 |
+                             *reinterpret_cast<const uint16_t*>(pb));
+  }
 };
 
-// Of a logit z: the smaller of sigmoid(z) and 1 - sigmoid(z), with z's sign; from it both follow
-// without cancellation.
-template <typename F> __device__ __forceinline__ F sigmoid_lower(F z) {
-  const F t = map_([](float v) { return ex2(-fabsf(v) * kLog2e); }, z);
-  const F r = map_(rcp, add_(t, all_<F>(1.f)));
-  return map_([](float l, float v) { return copysignf(l, v); }, mul_(t, r), z);
+__device__ __forceinline__ float rsqrt_(float x) {
+  float y;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
-template <typename F> __device__ __forceinline__ F sigmoid_of(F lo) {
-  return map_([](float l) { return signbit(l) ? -l : 1.f - l; }, lo);
-}
-template <typename F> __device__ __forceinline__ F one_minus_sigmoid_of(F lo) {
-  return map_([](float l) { return signbit(l) ? 1.f + l : l; }, lo);
-}
-
-// Makes the compiler forget what it computed from v: recomputing u, a^2, ... in the last walk is
-// cheaper than keeping them for all steps (they spilled).
-__device__ __forceinline__ void forget(float& v) { asm volatile("" : "+f"(v)); }
-__device__ __forceinline__ void forget(float2& v) { asm volatile("" : "+f"(v.x), "+f"(v.y)); }
 
 template <typename T, typename G, int V, bool LOGITS, bool RESET, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(32 * kBwdWarps, 2)
 glr_bwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __restrict__ beta,
                const float* __restrict__ decay, const uint8_t* __restrict__ reset,
                const float* __restrict__ ckpt, const T* __restrict__ dh,
@@ -426,17 +469,21 @@ glr_bwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
   using F = typename Lane<V>::F;
   using EX = Elem<T, V>;
   using EG = Elem<G, V>;
+  constexpr int N = kBwdSteps, WARPS = kBwdWarps;
   extern __shared__ __align__(16) uint8_t smem[];
   auto& ring = *reinterpret_cast<BwdRing<T, G, V>*>(smem);
-  __shared__ Maps<F, false> fwd_maps;
-  __shared__ Maps<F, CLUSTER> maps;
+  __shared__ Maps<F, WARPS, CLUSTER ? kBwdCluster : 1> maps;  // of R -> A R + Q
+  __shared__ F map_h[2][WARPS][32];                           // of s -> A s + H
   const Place p = place<V, CLUSTER>(C);
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int64_t tiles = (L + kTile - 1) / kTile, rounds = (tiles + p.size - 1) / p.size;
-  x += p.b * st.xb + p.c0;
-  g += p.b * st.gb + p.c0;
-  beta += p.b * st.bb + p.c0;
-  dh += p.b * L * C + p.c0;
+  const int lane = threadIdx.x & 31, w = warp_index();
+  const int64_t tiles = (L + kBwdTile - 1) / kBwdTile, rounds = (tiles + p.size - 1) / p.size;
+  const int64_t per_round = (int64_t)p.size * kBwdTile;
+  // the warp's first step of the round, from the last round to the first
+  int64_t t0 = ((rounds - 1) * p.size + p.rank) * kBwdTile + w * N;
+  Stream<T, V, N> in_x(x + p.b * st.xb + t0 * st.xl + p.c0, st.xl, -per_round * st.xl, C - p.c0, wide);
+  Stream<G, V, N> in_g(g + p.b * st.gb + t0 * st.gl + p.c0, st.gl, -per_round * st.gl, C - p.c0, wide);
+  Stream<G, V, N> in_b(beta + p.b * st.bb + t0 * st.bl + p.c0, st.bl, -per_round * st.bl, C - p.c0, wide);
+  Stream<T, V, N> in_d(dh + (p.b * L + t0) * C + p.c0, C, -per_round * C, C - p.c0, wide);
   if (RESET) reset += p.b * L;
   F rate = all_<F>(0.f), sum = all_<F>(0.f);
   F R = all_<F>(0.f);  // a_t D_t of the step behind the round
@@ -445,64 +492,67 @@ glr_bwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
       rate = map_([&](float d) { return -scale * softplus(d); }, Elem<float, V>::load(decay + p.c));
     if (dhT) R = Elem<float, V>::load(dhT + p.b * C + p.c);
   }
-  auto rows_of = [&](int64_t t0) { return t0 < L ? (int)(L - t0 < kSteps ? L - t0 : kSteps) : 0; };
-  auto fetch = [&](int64_t k) {  // k-th round from the end
-    const int64_t t0 = ((rounds - 1 - k) * p.size + p.rank) * kTile + w * kSteps;
-    const int s = (int)(k % kStages), n = k < rounds ? rows_of(t0) : 0;
-    if (n > 0) {
-      copy_rows<T, V>(ring.in.x[s][w], x + t0 * st.xl, st.xl, C - p.c0, n, wide);
-      copy_rows<G, V>(ring.in.g[s][w], g + t0 * st.gl, st.gl, C - p.c0, n, wide);
-      copy_rows<G, V>(ring.in.b[s][w], beta + t0 * st.bl, st.bl, C - p.c0, n, wide);
-      copy_rows<T, V>(ring.d[s][w], dh + t0 * C, C, C - p.c0, n, wide);
-    }
+  auto rows_of = [&](int64_t t) { return t >= 0 && t < L ? (int)(L - t < N ? L - t : N) : 0; };
+  int64_t t_fetch = t0;
+  auto fetch = [&](int stage) {
+    const int n = rows_of(t_fetch);  // 0 behind the end and in front of the first round
+    in_x.fetch(ring.x[stage][w], n);
+    in_d.fetch(ring.d[stage][w], n);
+    in_g.fetch(ring.g[stage][w], n);
+    in_b.fetch(ring.b[stage][w], n);
+    t_fetch -= per_round;
     copy_commit();
   };
 #pragma unroll
   for (int k = 0; k < kStages - 1; ++k) fetch(k);
-  for (int64_t k = 0; k < rounds; ++k) {
-    const int64_t tile = (rounds - 1 - k) * p.size + p.rank, t0 = tile * kTile + w * kSteps;
-    const int n = rows_of(t0), s = (int)(k % kStages);
-    F first = all_<F>(0.f);  // the state in front of the tile
-    if (p.on && tile < tiles) first = Elem<float, V>::load(ckpt + (p.b * tiles + tile) * C + p.c);
-    fetch(k + kStages - 1);
-    const uint32_t rs = RESET ? reset_bits(reset, t0, L) : 0;
+  int64_t o0 = (p.b * L + t0) * C + p.c0;  // of the slab in the warp's first row
+  const float* from = ckpt + (p.b * tiles + (rounds - 1) * p.size + p.rank) * C + p.c;
+  for (int64_t k = 0; k < rounds; ++k, t0 -= per_round, o0 -= per_round * C, from -= p.size * C) {
+    const int n = rows_of(t0), s = (int)(k % kStages), parity = (int)(k & 1);
+    F hv = all_<F>(0.f);  // the state in front of the tile
+    if (p.on && t0 - w * N < L) hv = Elem<float, V>::load(from);
+    fetch((int)((k + kStages - 1) % kStages));
+    const uint32_t rs = RESET ? reset_bits(reset, t0, n) : 0;
     copy_wait<kStages - 1>();
-    if (n < kSteps) {  // behind the end nothing comes in
+    if (n < N) {  // behind the end nothing comes in
       __syncwarp();
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i)
+      for (int i = 0; i < N; ++i)
         if (i >= n) {
-          EX::zero(&ring.in.x[s][w][i][lane * EX::kBytes]);
-          EX::zero(&ring.d[s][w][i][lane * EX::kBytes]);
-          EG::zero(&ring.in.g[s][w][i][lane * EG::kBytes]);
-          EG::zero(&ring.in.b[s][w][i][lane * EG::kBytes]);
+          EX::zero(&ring.x[s][w][(i * 32 + lane) * EX::kBytes]);
+          EX::zero(&ring.d[s][w][(i * 32 + lane) * EX::kBytes]);
+          EG::zero(&ring.g[s][w][(i * 32 + lane) * EG::kBytes]);
+          EG::zero(&ring.b[s][w][(i * 32 + lane) * EG::kBytes]);
         }
     }
     __syncwarp();
-    auto x_of = [&](int i) { return EX::load(&ring.in.x[s][w][i][lane * EX::kBytes]); };
-    auto beta_of = [&](int i) { return EG::load(&ring.in.b[s][w][i][lane * EG::kBytes]); };
-    auto d_of = [&](int i) { return EX::load(&ring.d[s][w][i][lane * EX::kBytes]); };
-    // What the walks need of the gates; x and dh are read again from the ring.
-    F a[kSteps], m[kSteps], lo_g[kSteps];  // values: only a
-    F(&lo_b)[kSteps][32] = ring.lo_b[w];
-    auto b_of = [&](int i) {
-      if (LOGITS) return mul_(mul_(m[i], sigmoid_of(lo_b[i][lane])), x_of(i));
-      return mul_(beta_of(i), x_of(i));
-    };
+    auto x_of = [&](int i) { return EX::load(&ring.x[s][w][(i * 32 + lane) * EX::kBytes]); };
+    auto d_of = [&](int i) { return EX::load(&ring.d[s][w][(i * 32 + lane) * EX::kBytes]); };
+    auto beta_of = [&](int i) { return EG::load(&ring.b[s][w][(i * 32 + lane) * EG::kBytes]); };
+    F a[N], u[N], c[N];  // u = log a and c = 1 - sigmoid(g) of logits
     F A = all_<F>(1.f), H = all_<F>(0.f), Q = all_<F>(0.f);
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      const F gv = EG::load(&ring.in.g[s][w][i][lane * EG::kBytes]);
+    for (int i = 0; i < N; ++i) {
+      const F gv = EG::load(&ring.g[s][w][(i * 32 + lane) * EG::kBytes]);
       F b;
       if (LOGITS) {
-        lo_g[i] = sigmoid_lower(gv);
-        const F lb = sigmoid_lower(beta_of(i));
-        lo_b[i][lane] = lb;
-        const F u = mul_(rate, sigmoid_of(lo_g[i]));
-        a[i] = map_(ex2, mul_(u, all_<F>(kLog2e)));
-        m[i] = map_(sqrt_, one_minus_exp(mul_(u, all_<F>(-2.f)), mul_(a[i], a[i])));
-        if (RESET && (rs >> i & 1)) m[i] = all_<F>(1.f);
-        b = mul_(mul_(m[i], sigmoid_of(lb)), x_of(i));
+        F sg, si, ci;
+        sigmoid_pair(gv, sg, c[i]);
+        sigmoid_pair(beta_of(i), si, ci);
+        u[i] = mul_(rate, sg);
+        a[i] = map_(ex2, mul_(u[i], all_<F>(kLog2e)));
+        const F a2 = mul_(a[i], a[i]);
+        // 1 - a^2, kept off 0: a == 1 leaves its limits, m = 0 and (a^2 / m) u = 0, to 1e-18
+        const F v = map_([](float t) { return fmaxf(t, 1e-36f); },
+                         one_minus_exp(mul_(u[i], all_<F>(-2.f)), a2));
+        const F rv = map_(rsqrt_, v);
+        F m = mul_(v, rv);
+        if (RESET && (rs >> i & 1)) m = all_<F>(1.f);
+        const F mi = mul_(m, si);
+        ring.q[w][i][lane] = mul_(a2, mul_(rv, rv));
+        ring.mi[w][i][lane] = mi;
+        ring.put_gates(s, w, i, lane, ci);
+        b = mul_(mi, x_of(i));
       } else {
         a[i] = gv;
         b = mul_(beta_of(i), x_of(i));
@@ -516,61 +566,52 @@ glr_bwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
       H = fma_(a[i], H, b);
     }
 #pragma unroll
-    for (int i = kSteps - 1; i >= 0; --i) {  // Q: D of step i, without what enters
-      if (i + 1 < kSteps) Q = RESET && (rs >> (i + 1) & 1) ? d_of(i) : fma_(a[i + 1], Q, d_of(i));
+    for (int i = N - 1; i >= 0; --i) {  // Q: D of step i, without what enters
+      if (i + 1 < N) Q = RESET && (rs >> (i + 1) & 1) ? d_of(i) : fma_(a[i + 1], Q, d_of(i));
       else Q = d_of(i);
     }
-    Q = RESET && (rs & 1) ? all_<F>(0.f) : mul_(a[0], Q);
-    F unused;
-    F hv = carry_in<F, false, false, RESET>(fwd_maps, (int)(k & 1), A, H, first, unused);
-    F d = carry_in<F, CLUSTER, true, RESET>(maps, (int)(k & 1), A, Q, R, unused);
+    maps.A[parity][w][lane] = finite(A);
+    maps.H[parity][w][lane] = RESET && (rs & 1) ? all_<F>(0.f) : mul_(a[0], Q);
+    map_h[parity][w][lane] = H;
+    __syncthreads();
+    F d = carry_in<true, RESET>(maps, parity, w, R);
+#pragma unroll 4
+    for (int q = 0; q < WARPS - 1; ++q)
+      if (q < w) hv = through<RESET>(hv, maps.A[parity][q][lane], map_h[parity][q][lane]);
     if (p.on) {
+      F D[N];
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        forget(a[i]);
-        if (LOGITS) {
-          forget(lo_g[i]);
-          forget(m[i]);
-        }
+      for (int i = N - 1; i >= 0; --i) {
+        if (i + 1 == N) d = add_(d, d_of(i));
+        else d = RESET && (rs >> (i + 1) & 1) ? d_of(i) : fma_(a[i + 1], d, d_of(i));
+        D[i] = d;
       }
-      F before[kSteps];
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        before[i] = hv;
-        if (RESET && (rs >> i & 1)) hv = all_<F>(0.f);
-        hv = fma_(a[i], hv, b_of(i));
-      }
-#pragma unroll
-      for (int i = 0; LOGITS && i < kSteps; ++i) forget(m[i]);
-      asm volatile("" ::: "memory");
-      int64_t o = (p.b * L + t0 + kSteps - 1) * C + p.c;
       auto walk = [&](auto full) {
+        int64_t o = o0 + lane * V;
 #pragma unroll
-        for (int i = kSteps - 1; i >= 0; --i, o -= C) {
+        for (int i = 0; i < N; ++i, o += C) {
           const bool zero = RESET && (rs >> i & 1);
           const F xv = x_of(i);
-          if (i + 1 == kSteps) d = add_(d, d_of(i));
-          else d = RESET && (rs >> (i + 1) & 1) ? d_of(i) : fma_(a[i + 1], d, d_of(i));
-          F ox, og, ob;
+          F ox, og, ob, b;
           if (LOGITS) {
-            const F u = mul_(rate, sigmoid_of(lo_g[i]));
-            const F lb = lo_b[i][lane];
-            const F mi = mul_(m[i], sigmoid_of(lb)), b = mul_(mi, xv);
-            // a^2 / (1 - a^2); a == 1 leaves the limit 0 of (that * u * b)
-            const F q = map_(
-                [](float m_, float v, float a2) { return m_ > 1e-18f ? a2 * rcp(v) : 0.f; }, m[i],
-                mul_(m[i], m[i]), mul_(a[i], a[i]));
-            F du = mul_(d, fma_(a[i], before[i], mul_(mul_(q, b), all_<F>(-1.f))));
+            const F mi = ring.mi[w][i][lane], ci = ring.get_gates(s, w, i, lane);
+            b = mul_(mi, xv);
+            F du = mul_(D[i], fma_(a[i], hv, mul_(mul_(ring.q[w][i][lane], b), all_<F>(-1.f))));
             if (zero) du = all_<F>(0.f);
-            if (full || i < n) sum = fma_(du, u, sum);
-            og = mul_(mul_(du, u), one_minus_sigmoid_of(lo_g[i]));
-            ox = mul_(d, mi);
-            ob = mul_(mul_(d, b), one_minus_sigmoid_of(lb));
+            du = mul_(du, u[i]);
+            if (full || i < n) sum = add_(sum, du);
+            og = mul_(du, c[i]);
+            ox = mul_(D[i], mi);
+            ob = mul_(mul_(D[i], b), ci);
           } else {
-            ox = mul_(d, beta_of(i));
-            ob = mul_(d, xv);
-            og = zero ? all_<F>(0.f) : mul_(d, before[i]);
+            const F be = beta_of(i);
+            b = mul_(be, xv);
+            ox = mul_(D[i], be);
+            ob = mul_(D[i], xv);
+            og = zero ? all_<F>(0.f) : mul_(D[i], hv);
           }
+          if (zero) hv = all_<F>(0.f);
+          hv = fma_(a[i], hv, b);
           if (full || i < n) {
             EX::store(dx + o, ox);
             EG::store(dg + o, og);
@@ -578,7 +619,7 @@ glr_bwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
           }
         }
       };
-      if (n == kSteps) walk(std::true_type{});
+      if (n == N) walk(std::true_type{});
       else walk(std::false_type{});
     }
     __syncwarp();
@@ -587,12 +628,12 @@ glr_bwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
   if (dh0 && p.on && p.rank == 0 && w == 0) Elem<float, V>::store(dh0 + p.b * C + p.c, R);
   if (LOGITS && ddecay_part) {
     __syncthreads();
-    fwd_maps.A[0][w][lane] = sum;
+    map_h[0][w][lane] = sum;
     __syncthreads();
     if (w == 0 && p.on) {
-      F t = fwd_maps.A[0][0][lane];
+      F t = map_h[0][0][lane];
 #pragma unroll
-      for (int k = 1; k < kWarps; ++k) t = add_(t, fwd_maps.A[0][k][lane]);
+      for (int k = 1; k < WARPS; ++k) t = add_(t, map_h[0][k][lane]);
       Elem<float, V>::store(ddecay_part + (p.b * p.size + p.rank) * C + p.c, t);
     }
   }
@@ -714,23 +755,22 @@ bool wide_ok(const void* const* xs, int nx, const void* const* gs, int ng, const
   return ok;
 }
 
-// CTAs of a cluster along time: doubled, up to 8 and up to the number of tiles, until there are
-// `want` CTAs.
-int cluster_for(int64_t ctas, int64_t L, int64_t want) {
-  const int64_t tiles = (L + kTile - 1) / kTile;
+// CTAs of a cluster along time: doubled, up to `most` and up to the number of tiles, until there
+// are `want` CTAs.
+int cluster_for(int64_t ctas, int64_t tiles, int64_t want, int most) {
   int n = 1;
-  while (n < 8 && ctas * n < want && 2 * n <= tiles) n *= 2;
+  while (n < most && ctas * n < want && 2 * n <= tiles) n *= 2;
   return n;
 }
 
 template <typename K, typename... Args>
-int launch(const char* what, K kernel, int64_t ctas, int cluster, int smem, cudaStream_t st,
+int launch(const char* what, K kernel, int64_t ctas, int cluster, int threads, int smem, cudaStream_t st,
            Args... args) {
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e == cudaSuccess) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(ctas * cluster));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr{};
@@ -775,11 +815,11 @@ extern "C" int fo_glr_fwd(const void* x, const void* g, const void* beta, const 
     const bool two = pairs_ok(xs, 2, gs, 2, fs, 4, q, C, sizeof(T), sizeof(G));
     const bool wide = wide_ok(xs, 1, gs, 2, q, C, sizeof(T), sizeof(G));
     const int64_t ctas = B * slabs_of(C, two ? 2 : 1);
-    const int cl = cluster_for(ctas, L, 2 * num_sms());
+    const int cl = cluster_for(ctas, (L + kFwdTile - 1) / kFwdTile, kFwdWant * num_sms(), kFwdCluster);
     return with_flags(two, decay, reset, cl > 1, [&](auto tw, auto lo, auto rs, auto c) {
       constexpr int V = tw && sizeof(G) == 2 ? 2 : 1;
       return launch("glr_fwd_kernel", glr_fwd_kernel<T, G, V, lo, rs, c>, ctas, cl,
-                    (int)sizeof(FwdRing<T, G, V>), as_stream(stream), (const T*)x, (const G*)g,
+                    32 * kFwdWarps, (int)sizeof(FwdRing<T, G, V>), as_stream(stream), (const T*)x, (const G*)g,
                     (const G*)beta, decay, h0, reset, (T*)h, hT, ckpt, L, C, s, scale, wide);
     });
   });
@@ -849,11 +889,11 @@ extern "C" int fo_glr_bwd(const void* x, const void* g, const void* beta, const 
     const bool two = pairs_ok(xs, 3, gs, 4, fs, 4, sq, C, sizeof(T), sizeof(G));
     const bool wide = wide_ok(xs, 2, gs, 2, sq, C, sizeof(T), sizeof(G));
     const int64_t ctas = B * slabs_of(C, two ? 2 : 1);
-    const int cl = cluster_for(ctas, L, 2 * num_sms());
+    const int cl = cluster_for(ctas, (L + kBwdTile - 1) / kBwdTile, kBwdWant * num_sms(), kBwdCluster);
     int rc = with_flags(two, decay, reset, cl > 1, [&](auto tw, auto lo, auto rs, auto c) {
       constexpr int V = tw && sizeof(G) == 2 ? 2 : 1;
       return launch("glr_bwd_kernel", glr_bwd_kernel<T, G, V, lo, rs, c>, ctas, cl,
-                    (int)sizeof(BwdRing<T, G, V>), q, (const T*)x, (const G*)g, (const G*)beta,
+                    32 * kBwdWarps, (int)sizeof(BwdRing<T, G, V>), q, (const T*)x, (const G*)g, (const G*)beta,
                     decay, reset, ckpt, (const T*)dh, dhT, (T*)dx, (G*)dg, (G*)dbeta, dh0, part,
                     L, C, s, scale, wide);
     });

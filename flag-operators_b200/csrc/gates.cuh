@@ -95,4 +95,12 @@ __device__ __forceinline__ float2 map_(Fn f, float2 a, float2 b, float2 c) {
   return make_float2(f(a.x, b.x, c.x), f(a.y, b.y, c.y));
 }
 
+// sigmoid(z) and 1 - sigmoid(z), neither with cancellation: e = e^-z, s = 1 / (1 + e), c = e s, which
+// is 1 (fmin passes over the NaN of inf * 0) where e is infinite.
+template <typename F> __device__ __forceinline__ void sigmoid_pair(F z, F& s, F& c) {
+  const F e = map_(ex2, mul_(z, all_<F>(-kLog2e)));
+  s = map_(rcp, add_(e, all_<F>(1.f)));
+  c = map_([](float v) { return fminf(v, 1.f); }, mul_(e, s));
+}
+
 }  // namespace fo

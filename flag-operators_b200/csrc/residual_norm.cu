@@ -235,14 +235,6 @@ __device__ __forceinline__ float inv_sqrt(float x) {
   return x < INFINITY ? r * fmaf(-0.5f * x * r, r, 1.5f) : r;
 }
 
-// sigmoid(z) and 1 - sigmoid(z) of pairs: e = e^-z, s = 1 / (1 + e), c = e s.  e is kept below
-// 2^126, so that e s is 1 (and s 1e-38 instead of 0) at the far end.
-__device__ __forceinline__ void sigmoid_pair(float2 z, float2& s, float2& c) {
-  const float2 e = map_([](float v) { return ex2(fminf(v, 126.f)); }, mul_(z, all_<float2>(-kLog2e)));
-  s = map_(rcp, add_(e, all_<float2>(1.f)));
-  c = mul_(e, s);
-}
-
 // Bytes of two fp32 weight vectors of N elements, each a multiple of 16.
 __host__ __device__ constexpr int weight_bytes(int64_t N) { return (int)((N + 3) / 4 * 4 * 8); }
 
