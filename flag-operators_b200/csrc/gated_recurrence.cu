@@ -68,6 +68,18 @@ __device__ __forceinline__ float sqrt_(float x) {
   return y;
 }
 
+__device__ __forceinline__ float rsqrt_(float x) {
+  float y;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// min that keeps a NaN
+__device__ __forceinline__ float min_nan(float x, float y) {
+  float z;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+  return z;
+}
+
 // softplus(decay), the rate of a fully open gate
 __device__ __forceinline__ float softplus(float decay) {
   return decay > 20.f ? decay : log1pf(expf(decay));
@@ -354,16 +366,18 @@ glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
       const F gv = EG::load(&ring.g[s][w][(i * 32 + lane) * EG::kBytes]);
       const F bv = EG::load(&ring.b[s][w][(i * 32 + lane) * EG::kBytes]);
       if (LOGITS) {
-        // 1 / (1 + e^-z): 0 and 1 at -inf and +inf
-        auto sig = [](F z) {
-          const F e = map_(ex2, mul_(z, all_<F>(-kLog2e)));
-          return map_(rcp, add_(e, all_<F>(1.f)));
-        };
-        const F sg = sig(gv);
+        // sigmoid(g) = 1 / (1 + e^-g), 0 and 1 at -inf and +inf; m i = sqrt(v) / q with v = 1 - a^2 and
+        // q = 1 + e^-beta (kept below 2^60) is v rsqrt(v q^2), which saves one of six of the slow
+        // instructions (exponentials, reciprocals, roots) that bound this kernel.
+        const F sg = map_(rcp, add_(map_(ex2, mul_(gv, all_<F>(-kLog2e))), all_<F>(1.f)));
         a[i] = map_(ex2, mul_(sg, r1));
-        F m = map_(sqrt_, one_minus_exp(mul_(sg, r2), mul_(a[i], a[i])));
-        if (RESET && (rs >> i & 1)) m = all_<F>(1.f);
-        b[i] = mul_(mul_(m, sig(bv)), xv);
+        F v = one_minus_exp(mul_(sg, r2), mul_(a[i], a[i]));
+        if (RESET && (rs >> i & 1)) v = all_<F>(1.f);
+        const F q = add_(map_([](float t) { return ex2(min_nan(t, 60.f)); }, mul_(bv, all_<F>(-kLog2e))),
+                         all_<F>(1.f));
+        // 1e-36: no root of 0 where a == 1, and v then makes the product 0
+        const F t = map_(rsqrt_, fma_(mul_(v, q), q, all_<F>(1e-36f)));
+        b[i] = mul_(mul_(v, t), xv);
       } else {
         a[i] = gv;
         b[i] = mul_(bv, xv);
@@ -451,12 +465,6 @@ template <typename T, typename G, int V> struct BwdRing {
                              *reinterpret_cast<const uint16_t*>(pb));
   }
 };
-
-__device__ __forceinline__ float rsqrt_(float x) {
-  float y;
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 template <typename T, typename G, int V, bool LOGITS, bool RESET, bool CLUSTER>
 __global__ void __launch_bounds__(32 * kBwdWarps, 2)
