@@ -80,32 +80,43 @@ emb_fwd_kernel(const I* __restrict__ ids, const T* __restrict__ w, T* __restrict
                int64_t V, int64_t N, int64_t ld, float scale, unsigned slabs) {
   using X = Vec<T, WIDE>;
   constexpr int K = WIDE ? 2 : 4;  // vectors of a thread in a row
-  const int64_t t0 = (int64_t)(blockIdx.x / slabs) * ROWS, nv = N / X::E;
-  const int64_t v0 = (int64_t)(blockIdx.x % slabs) * blockDim.x * K + threadIdx.x;
-  int64_t id[ROWS];
+  const int64_t t0 = (int64_t)(blockIdx.x / slabs) * ROWS;
+  const int v0 = (int)(blockIdx.x % slabs) * (int)blockDim.x * K + threadIdx.x;
+  const int left = (int)(N / X::E) - v0;  // vectors from the thread's first on
+  if (left <= 0) return;
+  // Offsets in W of the thread's first vector.  An id outside [0, V) is replaced before any address
+  // is made from it.
+  bool inside[ROWS];
+  int64_t from[ROWS];
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) id[r] = t0 + r < T_ ? (int64_t)ids[t0 + r] : -1;
+  for (int r = 0; r < ROWS; ++r) {
+    const int64_t id = t0 + r < T_ ? (int64_t)ids[t0 + r] : -1;
+    inside[r] = id >= 0 && id < V;
+    from[r] = (inside[r] ? id : 0) * ld + (int64_t)v0 * X::E;
+  }
   typename X::Raw raw[ROWS][K];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int64_t v = v0 + (int64_t)k * blockDim.x;
-      if (id[r] >= 0 && id[r] < V && v < nv) raw[r][k] = X::load(w + id[r] * ld + v * X::E);
-    }
+    for (int k = 0; k < K; ++k)
+      if (inside[r] && k * (int)blockDim.x < left)
+        raw[r][k] = X::load(w + from[r] + k * (int)blockDim.x * X::E);
+  T* to = out + t0 * N + (int64_t)v0 * X::E;
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r)
+  for (int r = 0; r < ROWS; ++r, to += N) {
+    if (t0 + r >= T_) break;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int64_t v = v0 + (int64_t)k * blockDim.x;
-      if (t0 + r < T_ && v < nv) {
-        float f[X::E];
-        X::unpack(raw[r][k], f);
+    for (int k = 0; k < K; ++k)
+      if (k * (int)blockDim.x < left) {
+        float f[X::E] = {};
+        if (inside[r]) {
+          X::unpack(raw[r][k], f);
 #pragma unroll
-        for (int e = 0; e < X::E; ++e) f[e] = id[r] >= 0 && id[r] < V ? f[e] * scale : 0.f;
-        X::store(out + (t0 + r) * N + v * X::E, f);
+          for (int e = 0; e < X::E; ++e) f[e] *= scale;
+        }
+        X::store(to + k * (int)blockDim.x * X::E, f);
       }
-    }
+  }
 }
 
 // A part of dW to be written as zeros by the CTAs of a kernel from `first_cta` on.
@@ -238,17 +249,34 @@ emb_merge_kernel(const int32_t* __restrict__ skey, const int32_t* __restrict__ s
                  Zeros zeros) {
   if (blockIdx.x >= zeros.first_cta) return write_zeros(zeros);
   constexpr int kAtOnce = 8;
+  // every kCoarse-th key of eight chunks, for the first half of their bisections
+  constexpr int kCoarse = 64, kMarks = kChunk / kCoarse;
+  __shared__ int32_t marks[kAtOnce][kMarks];
   const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i >= T) return;
-  const int t = (int)i, mine = t / kChunk;
+  const int t = (int)(i < T ? i : T - 1), mine = t / kChunk;
   const int32_t k = skey[t];
   int to = t - mine * kChunk;
   for (int c0 = 0; c0 < chunks; c0 += kAtOnce) {
+    __syncthreads();
+    for (int m = threadIdx.x; m < kAtOnce * kMarks; m += kThreads) {
+      const int64_t at = (int64_t)(c0 + m / kMarks) * kChunk + m % kMarks * kCoarse;
+      marks[m / kMarks][m % kMarks] = at < T ? skey[at] : INT32_MAX;
+    }
+    __syncthreads();
     int below[kAtOnce];
 #pragma unroll
     for (int q = 0; q < kAtOnce; ++q) below[q] = 0;
 #pragma unroll 1
-    for (int s = kChunk; s > 0; s >>= 1)
+    for (int s = kMarks; s > 0; s >>= 1)
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q) {
+        const int j = below[q] + s - 1;
+        if (j < kMarks && marks[q][j] < k + (c0 + q < mine)) below[q] += s;
+      }
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q) below[q] = below[q] ? (below[q] - 1) * kCoarse + 1 : 0;
+#pragma unroll 1
+    for (int s = kCoarse / 2; s > 0; s >>= 1)
 #pragma unroll
       for (int q = 0; q < kAtOnce; ++q) {
         const int c = c0 + q, j = below[q] + s - 1;
@@ -258,10 +286,13 @@ emb_merge_kernel(const int32_t* __restrict__ skey, const int32_t* __restrict__ s
           below[q] += s;
       }
 #pragma unroll
-    for (int q = 0; q < kAtOnce; ++q) to += below[q];
+    for (int q = 0; q < kAtOnce; ++q)
+      if (c0 + q < chunks && c0 + q != mine) to += below[q];
   }
-  key[to] = k;
-  pos[to] = spos[t];
+  if (i < T) {
+    key[to] = k;
+    pos[to] = spos[t];
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -269,16 +300,16 @@ emb_merge_kernel(const int32_t* __restrict__ skey, const int32_t* __restrict__ s
 // ---------------------------------------------------------------------------
 constexpr int kPiece = 32;   // sorted tokens of a piece
 constexpr int kRun = 16;     // pieces of a run
-constexpr int kUnroll = 8;   // rows of dout in flight a thread
 
 // A thread's columns of a row: one vector, or four elements blockDim.x apart.
 template <typename T, bool WIDE> struct Columns {
   using X = Vec<T, WIDE>;
   static constexpr int K = WIDE ? 1 : 4, E = X::E;
-  int64_t first, step, n;  // in vectors
+  int first, step, left;  // in vectors; left: from the first on
   float acc[K][E];
   __device__ __forceinline__ Columns(int64_t N, unsigned slab)
-      : first((int64_t)slab * blockDim.x * K + threadIdx.x), step(blockDim.x), n(N / E) {
+      : first((int)slab * (int)blockDim.x * K + (int)threadIdx.x), step((int)blockDim.x),
+        left((int)(N / E) - first) {
     clear();
   }
   __device__ __forceinline__ void clear() {
@@ -287,8 +318,8 @@ template <typename T, bool WIDE> struct Columns {
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[k][e] = 0.f;
   }
-  __device__ __forceinline__ bool on(int k) const { return first + k * step < n; }
-  __device__ __forceinline__ int64_t at(int k) const { return (first + k * step) * E; }
+  __device__ __forceinline__ bool on(int k) const { return k * step < left; }
+  __device__ __forceinline__ int at(int k) const { return (first + k * step) * E; }
   __device__ __forceinline__ void write(T* row, float scale) {
 #pragma unroll
     for (int k = 0; k < K; ++k)
@@ -314,6 +345,7 @@ emb_piece_kernel(const T* __restrict__ dout, const int32_t* __restrict__ key,
                  int T_, int64_t V, int64_t N, float scale, unsigned slabs) {
   using X = Vec<T, WIDE>;
   using Cols = Columns<T, WIDE>;
+  constexpr int kUnroll = WIDE ? 8 : 4;  // rows in flight a thread
   __shared__ int32_t pos_s[kPiece], key_s[kPiece + 2];  // keys from the one in front on
   const int64_t p = blockIdx.x / slabs;
   const int i0 = (int)(p * kPiece), n = T_ - i0 < kPiece ? T_ - i0 : kPiece;
@@ -389,11 +421,15 @@ emb_join_kernel(const int32_t* __restrict__ key, const float* __restrict__ part,
   const int32_t me = key[end - 1];
   if (me >= V || end >= T_ || key[end] != me) return;  // nothing goes on
   if (key[end - kPiece] == me && p > 0 && key[end - kPiece - 1] == me) return;  // began earlier
-  int lo = end, hi = T_;  // the last piece that has it: first sorted token behind, by bisection
+  // The first sorted token behind it: every warp splits [lo, hi] in 32 until it is found.
+  int lo = end, hi = T_;
   while (lo < hi) {
-    const int mid = lo + ((hi - lo) >> 1);
-    if (key[mid] <= me) lo = mid + 1;
-    else hi = mid;
+    const int step = (hi - lo + 31) / 32, at = lo + (int)(threadIdx.x & 31) * step;
+    const unsigned more = __ballot_sync(0xffffffffu, at < hi && key[at] <= me);
+    const int n = __popc(more);  // of the lanes' keys, that many are not behind it
+    const int top = lo + n * step;
+    if (n) lo = top - step + 1;
+    if (top < hi) hi = top;
   }
   const int q1 = (lo - 1) / kPiece + 1;  // behind the last piece
   Cols c(N, blockIdx.x % slabs);
@@ -436,9 +472,9 @@ int with_types(int dtype, int index_dtype, F&& f) {
 int check_sizes(int64_t T, int64_t V, int64_t N) {
   FO_CHECK_ARG(T >= 0 && V >= 0 && N >= 0, "embedding: negative size T=%lld V=%lld N=%lld",
                (long long)T, (long long)V, (long long)N);
-  const int64_t most = ((int64_t)1 << 31) - 1;
-  FO_CHECK_ARG(T <= most && V < most && N <= most,
-               "embedding: T=%lld, V=%lld and N=%lld must be below 2^31", (long long)T,
+  const int64_t most = (int64_t)1 << 30;
+  FO_CHECK_ARG(T <= most && V <= most && N <= most,
+               "embedding: T=%lld, V=%lld and N=%lld must not be over 2^30", (long long)T,
                (long long)V, (long long)N);
   return FO_OK;
 }

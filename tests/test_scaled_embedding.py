@@ -254,7 +254,7 @@ def test_c_entry_checks():
     P = 0x1000
     with pytest.raises(ValueError, match="negative size"):
         _lib.call("fo_embedding_fwd", P, P, P, -1, 4, 4, 4, 1.0, 0, 5, None)
-    with pytest.raises(ValueError, match="below 2\\^31"):
+    with pytest.raises(ValueError, match="over 2\\^30"):
         _lib.call("fo_embedding_fwd", P, P, P, 1 << 31, 4, 4, 4, 1.0, 0, 5, None)
     with pytest.raises(ValueError, match="null pointer"):
         _lib.call("fo_embedding_fwd", None, P, P, 1, 4, 4, 4, 1.0, 0, 5, None)
