@@ -24,7 +24,8 @@
 // and each warp then walks its steps once from the state that enters them.  So the axis is
 // walked 64 steps at a time and every input is read once.  Where B * C gives too few CTAs to fill
 // the GPU, up to 8 CTAs of a cluster take consecutive tiles and exchange their maps through
-// distributed shared memory, one cluster barrier a round.  The next tiles' inputs are on their way
+// distributed shared memory, as asynchronous stores that an mbarrier of the receiver counts (a cluster
+// barrier would wait for the outputs' stores too: 104 against TIME us at 1 x 16384 x 2048 bf16).  The next tiles' inputs are on their way
 // meanwhile: a ring of kStages tiles in shared memory, each thread copying (cp.async) just the
 // elements that it will read, so that the ring needs no barrier.
 #include <type_traits>
@@ -38,12 +39,10 @@ constexpr int kFwdSteps = 16, kFwdWarps = 8;  // steps of a thread in a round, a
 constexpr int kFwdTile = kFwdSteps * kFwdWarps;
 constexpr int kBwdSteps = 8, kBwdWarps = 8;
 constexpr int kBwdTile = kBwdSteps * kBwdWarps;
-constexpr int kBwdCluster = 4;                // CTAs of a cluster, at most
-constexpr int kFwdCluster = 8;
-constexpr int kFwdWant = 1, kBwdWant = 1;     // CTAs an SM below which clusters are made
+constexpr int kMostCtas = 8;                   // of a cluster
 constexpr int kStages = 2;                 // tiles of the ring
 static_assert(kBwdTile == FO_GLR_CHECKPOINT, "a tile of the backward begins at a checkpoint");
-static_assert(kFwdCluster <= kFwdWarps && kBwdCluster <= kBwdWarps, "a warp for each CTA");
+static_assert(kMostCtas <= kFwdWarps && kMostCtas <= kBwdWarps, "a warp for each CTA");
 static_assert(FO_GLR_CHECKPOINT % kFwdSteps == 0, "a warp's steps begin at a checkpoint or have none");
 
 struct Strides {
@@ -201,37 +200,85 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
                    : "memory");
 }
-__device__ __forceinline__ void store_remote(void* smem, uint32_t cta, float v) {
+__device__ __forceinline__ uint32_t shared_address(const void* p) {
+  return (uint32_t)__cvta_generic_to_shared(p);
+}
+__device__ __forceinline__ uint32_t remote_address(const void* p, uint32_t cta) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(shared_address(p)), "r"(cta));
+  return r;
+}
+// Two values into CTA `cta`'s copy of `to`, counted by its copy of `bar`
+__device__ __forceinline__ void send(void* to, const uint64_t* bar, uint32_t cta, float a, float h) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(
+                   remote_address(to, cta)),
+               "f"(a), "f"(h), "r"(remote_address(bar, cta))
+               : "memory");
+}
+__device__ __forceinline__ void send(void* to, const uint64_t* bar, uint32_t cta, float2 a, float2 h) {
   asm volatile(
-      "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, %1;\n\t"
-      "st.shared::cluster.f32 [r], %2;\n\t}" ::"r"((uint32_t)__cvta_generic_to_shared(smem)),
-      "r"(cta), "f"(v)
+      "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(
+          remote_address(to, cta)),
+      "f"(a.x), "f"(a.y), "f"(h.x), "f"(h.y), "r"(remote_address(bar, cta))
       : "memory");
 }
-__device__ __forceinline__ void store_remote(void* smem, uint32_t cta, float2 v) {
-  asm volatile(
-      "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, %1;\n\t"
-      "st.shared::cluster.v2.f32 [r], {%2, %3};\n\t}" ::"r"((uint32_t)__cvta_generic_to_shared(smem)),
-      "r"(cta), "f"(v.x), "f"(v.y)
-      : "memory");
+__device__ unsigned int g_glr_timeouts = 0;
+constexpr int kMaxPolls = 1 << 22;
+// Waits for phase `parity` of the mbarrier; gives up (and says so) after kMaxPolls polls.
+__device__ __forceinline__ bool wait_phase(const uint64_t* bar, uint32_t parity) {
+  for (int i = 0; i < kMaxPolls; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(shared_address(bar)), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  return false;
 }
 
 // The maps of a round: of the CTA's warps, and (clusters) of the cluster's CTAs.  Two copies,
-// used in turn: a copy is written again only after a barrier that every reader of it has passed.
+// used in turn.  One of the CTA is written again only behind a barrier that every reader of it has
+// passed; one of the cluster only by CTAs that have what this one sent after its readers' last
+// __syncthreads.
 template <typename F, int WARPS, int CTAS> struct Maps {
+  struct alignas(2 * sizeof(F)) Both {
+    F A, H;
+  };
   F A[2][WARPS][32], H[2][WARPS][32];
-  F cA[2][CTAS][32], cH[2][CTAS][32];
+  Both cta[2][CTAS][32];
+  uint64_t bar[2];
+  bool dead;
+
+  __device__ __forceinline__ void init() {
+    if constexpr (CTAS > 1) {
+      if (threadIdx.x == 0) {
+        dead = false;
+        for (int k = 0; k < 2; ++k)
+          asm volatile("mbarrier.init.shared.b64 [%0], 1;" ::"r"(shared_address(&bar[k])) : "memory");
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      }
+      cluster_barrier();
+    }
+  }
 };
 
-// With the maps of all warps in place, and the state S in front of the round: the state in front of
-// warp w's steps; S becomes the state behind the round.  REVERSE walks the warps and CTAs from the
-// last to the first.
+// With the maps of all warps in place, and the state S in front of round number `round`: the state
+// in front of warp w's steps; S becomes the state behind the round.  REVERSE walks the warps and CTAs
+// from the last to the first.
 template <bool REVERSE, bool RESET, typename F, int WARPS, int CTAS>
-__device__ __forceinline__ F carry_in(Maps<F, WARPS, CTAS>& m, int parity, int w, F& S) {
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ F carry_in(Maps<F, WARPS, CTAS>& m, int64_t round, int w, F& S) {
+  const int lane = threadIdx.x & 31, parity = (int)(round & 1);
   F mine = S;
   if constexpr (CTAS > 1) {
     const uint32_t n = cluster_size(), me = cluster_rank();
+    if (threadIdx.x == 0)
+      asm volatile("mbarrier.arrive.expect_tx.shared.b64 _, [%0], %1;" ::"r"(shared_address(&m.bar[parity])),
+                   "r"(n * 32 * (uint32_t)sizeof(typename Maps<F, WARPS, CTAS>::Both))
+                   : "memory");
     if (w < (int)n) {  // warp w hands the CTA's map to CTA w
       F a = all_<F>(1.f), h = all_<F>(0.f);
 #pragma unroll
@@ -241,14 +288,16 @@ __device__ __forceinline__ F carry_in(Maps<F, WARPS, CTAS>& m, int parity, int w
         h = through<RESET>(h, ak, m.H[parity][q][lane]);
         a = finite(mul_(a, ak));
       }
-      store_remote(&m.cA[parity][me][lane], w, a);
-      store_remote(&m.cH[parity][me][lane], w, h);
+      send(&m.cta[parity][me][lane], &m.bar[parity], w, a, h);
     }
-    cluster_barrier();
+    if (!m.dead && !wait_phase(&m.bar[parity], (uint32_t)(round >> 1) & 1)) {
+      m.dead = true;  // no further waits: the kernel ends, its outputs are not complete
+      atomicAdd(&g_glr_timeouts, 1u);
+    }
     for (uint32_t k = 0; k < n; ++k) {
       const uint32_t q = REVERSE ? n - 1 - k : k;
       if (q == me) mine = S;
-      S = through<RESET>(S, m.cA[parity][q][lane], m.cH[parity][q][lane]);
+      S = through<RESET>(S, m.cta[parity][q][lane].A, m.cta[parity][q][lane].H);
     }
 #pragma unroll
     for (int k = 0; k < WARPS - 1; ++k) {
@@ -305,7 +354,7 @@ template <typename T, typename G, int V> struct FwdRing {
   uint8_t b[kStages][kFwdWarps][Stream<G, V, kFwdSteps>::kBytes];
 };
 
-template <typename T, typename G, int V, bool LOGITS, bool RESET, bool CLUSTER>
+template <typename T, typename G, int V, bool LOGITS, bool RESET, int CTAS>
 __global__ void __launch_bounds__(32 * kFwdWarps, 2)
 glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __restrict__ beta,
                const float* __restrict__ decay, const float* __restrict__ h0,
@@ -317,8 +366,9 @@ glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
   constexpr int N = kFwdSteps;
   extern __shared__ __align__(16) uint8_t smem[];
   auto& ring = *reinterpret_cast<FwdRing<T, G, V>*>(smem);
-  __shared__ Maps<F, kFwdWarps, CLUSTER ? kFwdCluster : 1> maps;
-  const Place p = place<V, CLUSTER>(C);
+  __shared__ Maps<F, kFwdWarps, CTAS> maps;
+  maps.init();
+  const Place p = place<V, (CTAS > 1)>(C);
   const int lane = threadIdx.x & 31, w = warp_index();
   const int64_t tiles = (L + kFwdTile - 1) / kFwdTile, rounds = (tiles + p.size - 1) / p.size;
   const int64_t checkpoints = (L + FO_GLR_CHECKPOINT - 1) / FO_GLR_CHECKPOINT;
@@ -402,7 +452,7 @@ glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
     maps.A[parity][w][lane] = finite(A);
     maps.H[parity][w][lane] = H;
     __syncthreads();
-    F hv = carry_in<false, RESET>(maps, parity, w, S);
+    F hv = carry_in<false, RESET>(maps, round, w, S);
     if (p.on) {
       if (ckpt && n > 0 && t0 % FO_GLR_CHECKPOINT == 0)
         Elem<float, V>::store(ckpt + (p.b * checkpoints + t0 / FO_GLR_CHECKPOINT) * C + p.c, hv);
@@ -466,7 +516,7 @@ template <typename T, typename G, int V> struct BwdRing {
   }
 };
 
-template <typename T, typename G, int V, bool LOGITS, bool RESET, bool CLUSTER>
+template <typename T, typename G, int V, bool LOGITS, bool RESET, int CTAS>
 __global__ void __launch_bounds__(32 * kBwdWarps, 2)
 glr_bwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __restrict__ beta,
                const float* __restrict__ decay, const uint8_t* __restrict__ reset,
@@ -480,9 +530,10 @@ glr_bwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
   constexpr int N = kBwdSteps, WARPS = kBwdWarps;
   extern __shared__ __align__(16) uint8_t smem[];
   auto& ring = *reinterpret_cast<BwdRing<T, G, V>*>(smem);
-  __shared__ Maps<F, WARPS, CLUSTER ? kBwdCluster : 1> maps;  // of R -> A R + Q
-  __shared__ F map_h[2][WARPS][32];                           // of s -> A s + H
-  const Place p = place<V, CLUSTER>(C);
+  __shared__ Maps<F, WARPS, CTAS> maps;  // of R -> A R + Q
+  __shared__ F map_h[2][WARPS][32];      // of s -> A s + H
+  maps.init();
+  const Place p = place<V, (CTAS > 1)>(C);
   const int lane = threadIdx.x & 31, w = warp_index();
   const int64_t tiles = (L + kBwdTile - 1) / kBwdTile, rounds = (tiles + p.size - 1) / p.size;
   const int64_t per_round = (int64_t)p.size * kBwdTile;
@@ -582,7 +633,7 @@ glr_bwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
     maps.H[parity][w][lane] = RESET && (rs & 1) ? all_<F>(0.f) : mul_(a[0], Q);
     map_h[parity][w][lane] = H;
     __syncthreads();
-    F d = carry_in<true, RESET>(maps, parity, w, R);
+    F d = carry_in<true, RESET>(maps, k, w, R);
 #pragma unroll 4
     for (int q = 0; q < WARPS - 1; ++q)
       if (q < w) hv = through<RESET>(hv, maps.A[parity][q][lane], map_h[parity][q][lane]);
@@ -713,16 +764,13 @@ int with_types(int dtype, int gate_dtype, F&& f) {
   return FO_EDTYPE;
 }
 
-// Calls f with two integral constants: v == 1 or 2, and three truth values.
-template <typename F>
-int with_flags(bool two, bool logits, bool reset, bool cluster, F&& f) {
+// Calls f with three truth values as constants.
+template <typename F> int with_flags(bool two, bool logits, bool reset, F&& f) {
   auto b = [](bool v, auto&& k) {
     return v ? k(std::true_type{}) : k(std::false_type{});
   };
   return b(two, [&](auto t) {
-    return b(logits, [&](auto l) {
-      return b(reset, [&](auto r) { return b(cluster, [&](auto c) { return f(t, l, r, c); }); });
-    });
+    return b(logits, [&](auto l) { return b(reset, [&](auto r) { return f(t, l, r); }); });
   });
 }
 
@@ -823,12 +871,18 @@ extern "C" int fo_glr_fwd(const void* x, const void* g, const void* beta, const 
     const bool two = pairs_ok(xs, 2, gs, 2, fs, 4, q, C, sizeof(T), sizeof(G));
     const bool wide = wide_ok(xs, 1, gs, 2, q, C, sizeof(T), sizeof(G));
     const int64_t ctas = B * slabs_of(C, two ? 2 : 1);
-    const int cl = cluster_for(ctas, (L + kFwdTile - 1) / kFwdTile, kFwdWant * num_sms(), kFwdCluster);
-    return with_flags(two, decay, reset, cl > 1, [&](auto tw, auto lo, auto rs, auto c) {
+    // CTAs of a cluster until every SM has one: 266 us without, 294 with two at 8 x 8192 x 2048 bf16,
+    // where there are 256 CTAs as it is.
+    const int cl = cluster_for(ctas, (L + kFwdTile - 1) / kFwdTile, num_sms(), kMostCtas);
+    return with_flags(two, decay, reset, [&](auto tw, auto lo, auto rs) {
       constexpr int V = tw && sizeof(G) == 2 ? 2 : 1;
-      return launch("glr_fwd_kernel", glr_fwd_kernel<T, G, V, lo, rs, c>, ctas, cl,
-                    32 * kFwdWarps, (int)sizeof(FwdRing<T, G, V>), as_stream(stream), (const T*)x, (const G*)g,
-                    (const G*)beta, decay, h0, reset, (T*)h, hT, ckpt, L, C, s, scale, wide);
+      auto run = [&](auto kernel) {
+        return launch("glr_fwd_kernel", kernel, ctas, cl, 32 * kFwdWarps,
+                      (int)sizeof(FwdRing<T, G, V>), as_stream(stream), (const T*)x, (const G*)g,
+                      (const G*)beta, decay, h0, reset, (T*)h, hT, ckpt, L, C, s, scale, wide);
+      };
+      return cl > 1 ? run(glr_fwd_kernel<T, G, V, lo, rs, kMostCtas>)
+                    : run(glr_fwd_kernel<T, G, V, lo, rs, 1>);
     });
   });
 }
@@ -890,6 +944,7 @@ extern "C" int fo_glr_bwd(const void* x, const void* g, const void* beta, const 
   const int64_t* sq = strides ? strides : kZeroStrides;
   const Strides s{sq[0], sq[1], sq[2], sq[3], sq[4], sq[5]};
   float* part = ddecay ? (float*)workspace : nullptr;
+  int cl = 1;
   return with_types(dtype, gate_dtype, [&](auto t, auto gt) {
     using T = decltype(t);
     using G = decltype(gt);
@@ -897,16 +952,32 @@ extern "C" int fo_glr_bwd(const void* x, const void* g, const void* beta, const 
     const bool two = pairs_ok(xs, 3, gs, 4, fs, 4, sq, C, sizeof(T), sizeof(G));
     const bool wide = wide_ok(xs, 2, gs, 2, sq, C, sizeof(T), sizeof(G));
     const int64_t ctas = B * slabs_of(C, two ? 2 : 1);
-    const int cl = cluster_for(ctas, (L + kBwdTile - 1) / kBwdTile, kBwdWant * num_sms(), kBwdCluster);
-    int rc = with_flags(two, decay, reset, cl > 1, [&](auto tw, auto lo, auto rs, auto c) {
+    // Clusters of 8 leave room for one CTA on an SM instead of two, so they are for few CTAs: 372 us
+    // with 4, 202 with 8 at 1 x 32768 x 512 bf16 (8 slabs), 56 and 88 us at 2 x 4096 x 1024 (32).
+    const int most = ctas * kMostCtas <= num_sms() ? kMostCtas : 4;
+    cl = cluster_for(ctas, (L + kBwdTile - 1) / kBwdTile, num_sms(), most);
+    int rc = with_flags(two, decay, reset, [&](auto tw, auto lo, auto rs) {
       constexpr int V = tw && sizeof(G) == 2 ? 2 : 1;
-      return launch("glr_bwd_kernel", glr_bwd_kernel<T, G, V, lo, rs, c>, ctas, cl,
-                    32 * kBwdWarps, (int)sizeof(BwdRing<T, G, V>), q, (const T*)x, (const G*)g, (const G*)beta,
-                    decay, reset, ckpt, (const T*)dh, dhT, (T*)dx, (G*)dg, (G*)dbeta, dh0, part,
-                    L, C, s, scale, wide);
+      auto run = [&](auto kernel) {
+        return launch("glr_bwd_kernel", kernel, ctas, cl, 32 * kBwdWarps,
+                      (int)sizeof(BwdRing<T, G, V>), q, (const T*)x, (const G*)g, (const G*)beta,
+                      decay, reset, ckpt, (const T*)dh, dhT, (T*)dx, (G*)dg, (G*)dbeta, dh0, part,
+                      L, C, s, scale, wide);
+      };
+      return cl > 4   ? run(glr_bwd_kernel<T, G, V, lo, rs, 8>)
+             : cl > 1 ? run(glr_bwd_kernel<T, G, V, lo, rs, 4>)
+                      : run(glr_bwd_kernel<T, G, V, lo, rs, 1>);
     });
     if (rc || !ddecay) return rc;
     glr_ddecay_kernel<<<(unsigned)((C + 127) / 128), 128, 0, q>>>(part, B * cl, decay, ddecay, C);
     return check_launch("glr_ddecay_kernel");
   });
+}
+
+extern "C" int fo_glr_timeouts(unsigned int* count) {
+  clear_error();
+  FO_CHECK_ARG(count, "fo_glr_timeouts: null pointer");
+  if (cudaMemcpyFromSymbol(count, g_glr_timeouts, sizeof(unsigned int)) != cudaSuccess)
+    return check_launch("fo_glr_timeouts");
+  return FO_OK;
 }

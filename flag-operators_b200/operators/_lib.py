@@ -89,6 +89,7 @@ _SIGS = {
     "fo_glr_bwd_workspace_bytes": [_i64, _i64, _i64, _i64p],
     "fo_glr_bwd": [_c_void_p] * 13 + [_i64, _i64, _i64, _i64p, _f32, _int, _int, _c_void_p, _i64,
                                       _c_void_p],
+    "fo_glr_timeouts": [_c_void_p],
     "fo_residual_rms_norm_fwd": [_c_void_p] * 6 + [_f32] + [_c_void_p] * 4 + [_i64] * 5 + [
         _f32, _int, _int, _int, _c_void_p],
     "fo_residual_rms_norm_bwd_workspace_bytes": [_i64, _i64, _i64p],

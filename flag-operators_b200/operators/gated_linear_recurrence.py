@@ -203,3 +203,10 @@ def gated_linear_recurrence_step(
                   _lib.ptr(state), _lib.ptr(h), B, C, _strides(x, g, beta), float(decay_scale),
                   _lib.dtype_code(x.dtype), _lib.dtype_code(g.dtype), _lib.stream_of(x))
     return h
+
+
+def timeouts() -> int:
+    """Waits between CTAs that ran out of polls since the library was loaded (0 in a healthy run)."""
+    c = ctypes.c_uint(0)
+    _lib.call("fo_glr_timeouts", ctypes.byref(c))
+    return int(c.value)

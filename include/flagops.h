@@ -425,6 +425,11 @@ FO_API int fo_glr_bwd(const void* x, const void* g, const void* beta, const floa
                       int64_t L, int64_t C, const int64_t* strides, float scale, int dtype,
                       int gate_dtype, void* workspace, int64_t ws_bytes, void* stream);
 
+/* Number of waits between the CTAs of a cluster that ran out of polls since the library was loaded
+ * (0 in a healthy run; such a call's outputs are not complete).  Synchronous read of a device
+ * counter. */
+FO_API int fo_glr_timeouts(unsigned int* count);
+
 /* ------------------------------------------------------------------------ */
 /* residual RMS norm (no reference counterpart)                              */
 /* ------------------------------------------------------------------------ */

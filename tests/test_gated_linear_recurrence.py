@@ -14,7 +14,7 @@ import torch
 
 from operators import _lib
 from operators.gated_linear_recurrence import (gated_linear_recurrence,
-                                               gated_linear_recurrence_step)
+                                               gated_linear_recurrence_step, timeouts)
 
 DEV = "cuda"
 U = 2.0 ** -24
@@ -433,6 +433,12 @@ def test_captured_forward_and_backward_replay():
     graph.replay()
     want = _run(v2, 8.0)
     assert all(torch.equal(o, want[k]) for k, o in zip(names, out))
+
+
+@gpu
+def test_no_wait_timed_out():
+    _check(_inputs(1, 5000, 64, torch.bfloat16, torch.bfloat16, True, reset=0.01))
+    assert timeouts() == 0
 
 
 @gpu
