@@ -33,6 +33,10 @@ inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s
 // Number of SMs of the current device (cached per device).
 int num_sms();
 
+// Raises a kernel's dynamic shared memory limit on the current device to `bytes`, which has to be
+// the same in every call for a kernel; once only (the runtime's call costs about a microsecond).
+cudaError_t allow_shared(const void* kernel, int bytes);
+
 // ---------------------------------------------------------------------------
 // Scalar conversions
 // ---------------------------------------------------------------------------

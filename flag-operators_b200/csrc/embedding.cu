@@ -598,8 +598,7 @@ extern "C" int fo_embedding_bwd(const void* dout, const void* ids, void* dw, int
     const int64_t first = chunks > 1 ? bytes / 4 * 3 / 256 * 256 : bytes;
     int bits = 0;
     while (bits < 31 && V >> bits) ++bits;
-    cudaError_t e = cudaFuncSetAttribute(
-        emb_sort_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SortSmem));
+    cudaError_t e = allow_shared((const void*)emb_sort_kernel<I>, (int)sizeof(SortSmem));
     if (e != cudaSuccess) {
       cudaGetLastError();
       set_error("emb_sort_kernel: %s", cudaGetErrorString(e));

@@ -822,7 +822,7 @@ int cluster_for(int64_t ctas, int64_t tiles, int64_t want, int most) {
 template <typename K, typename... Args>
 int launch(const char* what, K kernel, int64_t ctas, int cluster, int threads, int smem, cudaStream_t st,
            Args... args) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_shared((const void*)kernel, smem);
   if (e == cudaSuccess) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(ctas * cluster));

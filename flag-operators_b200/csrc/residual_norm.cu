@@ -738,7 +738,7 @@ template <typename K, typename A>
 int launch(const char* what, K kernel, int64_t ctas, int threads, int smem, const A& a,
            cudaStream_t st) {
   if (smem > 40 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = allow_shared((const void*)kernel, 227 * 1024 - 1024);
     if (e != cudaSuccess) {
       cudaGetLastError();
       set_error("%s: %s", what, cudaGetErrorString(e));

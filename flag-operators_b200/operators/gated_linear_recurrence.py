@@ -54,9 +54,9 @@ def _check_gates(op, x, g, beta, decay):
         raise TypeError(f"{op}: dtype {x.dtype} is not supported")
     if decay is not None and decay.shape != x.shape[-1:]:
         raise ValueError(f"{op}: decay shape {tuple(decay.shape)}, expected ({x.shape[-1]},)")
-    for name, t in (("g", g), ("beta", beta), ("decay", decay)):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{op}: {name} must be on the same device as x")
+    dev = x.device
+    if g.device != dev or beta.device != dev or (decay is not None and decay.device != dev):
+        raise ValueError(f"{op}: g, beta and decay must be on the same device as x")
 
 
 def _rows(t):
@@ -64,8 +64,13 @@ def _rows(t):
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
-def _strides(*ts):
-    return _lib.i64_array([s for t in ts for s in t.stride()[:-1]])
+_Three, _Six = ctypes.c_int64 * 3, ctypes.c_int64 * 6
+
+
+def _strides(x, g, beta):
+    if x.dim() == 2:
+        return _Three(x.stride(0), g.stride(0), beta.stride(0))
+    return _Six(x.stride(0), x.stride(1), g.stride(0), g.stride(1), beta.stride(0), beta.stride(1))
 
 
 def _forward(x, g, beta, decay, h0, reset, scale, want_state, want_ckpt):
@@ -96,7 +101,7 @@ def _backward(x, g, beta, decay, reset, ckpt, scale, dh, dhT, need_dh0, need_dde
     with _lib.on_device(x):
         if need_ddecay:
             _lib.call("fo_glr_bwd_workspace_bytes", B, L, C, ctypes.byref(nbytes))
-            ws = torch.empty(max(nbytes.value, 1), dtype=torch.uint8, device=dev)
+            ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
         _lib.call("fo_glr_bwd", _lib.ptr(x), _lib.ptr(g), _lib.ptr(beta), _lib.ptr(decay),
                   _lib.ptr(reset), _lib.ptr(ckpt), _lib.ptr(dh), _lib.ptr(dhT), _lib.ptr(dx),
                   _lib.ptr(dg), _lib.ptr(dbeta), _lib.ptr(dh0), _lib.ptr(ddecay), B, L, C,
@@ -162,8 +167,9 @@ def gated_linear_recurrence(
         decay = decay.to(torch.float32).contiguous()
     x, g, beta = _rows(x), _rows(g), _rows(beta)
     scale = float(decay_scale)
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, g, beta, decay, h0)):
+    if torch.is_grad_enabled() and (x.requires_grad or g.requires_grad or beta.requires_grad
+                                    or (decay is not None and decay.requires_grad)
+                                    or (h0 is not None and h0.requires_grad)):
         return _GatedLinearRecurrence.apply(x, g, beta, decay, h0, reset, scale,
                                             bool(output_final_state))
     h, hT, _ = _forward(x, g, beta, decay, h0, reset, scale, output_final_state, False)
@@ -189,8 +195,9 @@ def gated_linear_recurrence_step(
             or not state.is_contiguous():
         raise ValueError(f"{op}: state must be a contiguous float32 tensor of shape {tuple(x.shape)} on "
                          f"x's device, got {state.dtype} {tuple(state.shape)} on {state.device}")
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, g, beta, state, decay)):
+    if torch.is_grad_enabled() and (x.requires_grad or g.requires_grad or beta.requires_grad
+                                    or state.requires_grad
+                                    or (decay is not None and decay.requires_grad)):
         raise RuntimeError(f"{op}: overwrites its state and is not differentiable; call it under "
                            f"torch.no_grad() or use gated_linear_recurrence")
     if decay is not None:

@@ -436,6 +436,33 @@ def test_captured_forward_and_backward_replay():
 
 
 @gpu
+def test_offsets_over_32_bits():
+    """2.2e9 elements: the last steps of the whole sequence, and of its tail from the state in front
+    of it.  The tiles lie otherwise, so both carry the bound of their own way: E of h is at most
+    20 U (H + 1) a step over the memory of the gates (values of at most 0.95: 20 steps), so they are
+    within 2 * 20 * 20 U * 4 = 1e-4 of each other in fp32; h and the gradients add a step of bf16."""
+    L, C, cut = (1 << 20) + 77, 2050, (1 << 20) - 200
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randn(1, L, C, device=DEV, generator=gen, dtype=torch.bfloat16)
+    g = torch.rand(1, L, C, device=DEV, generator=gen, dtype=torch.bfloat16).mul_(0.95)
+    assert x.numel() > 1 << 31
+    leaf = x.requires_grad_()
+    h, hT = gated_linear_recurrence(leaf, g, g, output_final_state=True)
+    with torch.no_grad():
+        _, front = gated_linear_recurrence(leaf[:, :cut], g[:, :cut], g[:, :cut], output_final_state=True)
+    tail = leaf.detach()[:, cut:].clone().requires_grad_()
+    gt = g[:, cut:]
+    ht, hTt = gated_linear_recurrence(tail, gt, gt, initial_state=front, output_final_state=True)
+    torch.testing.assert_close(hT, hTt, rtol=0, atol=1e-4)
+    torch.testing.assert_close(h[:, cut:], ht, rtol=2 ** -7, atol=1e-4)
+    ones = torch.ones_like(hT)
+    (dx,) = torch.autograd.grad((h, hT), [leaf], (x.detach(), ones))
+    (dt,) = torch.autograd.grad((ht, hTt), [tail], (tail.detach(), ones))
+    torch.testing.assert_close(dx[:, cut:], dt, rtol=2 ** -7, atol=1e-4)
+    assert bool(torch.isfinite(dx[:, ::4099]).all())
+
+
+@gpu
 def test_no_wait_timed_out():
     _check(_inputs(1, 5000, 64, torch.bfloat16, torch.bfloat16, True, reset=0.01))
     assert timeouts() == 0

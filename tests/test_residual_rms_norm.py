@@ -271,6 +271,23 @@ def test_empty_and_repeatable():
 
 
 @gpu
+def test_offsets_over_32_bits():
+    """2.2e9 elements: rows do not depend on one another, so the last ones equal those of a call of
+    their own, bit for bit."""
+    M, N = 262144 + 301, 8192
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    r = lambda *s: torch.randn(*s, device=DEV, generator=gen, dtype=torch.bfloat16)  # noqa: E731
+    y, w = r(M, N).requires_grad_(), r(N)
+    assert y.numel() > 1 << 31
+    out, res = residual_rms_norm(y, y.detach(), w, post_weight=w, gate=y.detach(), scale=w)
+    (dy,) = torch.autograd.grad((out, res), [y], (y.detach(), y.detach()))
+    t = y.detach()[-400:].clone().requires_grad_()
+    o2, r2 = residual_rms_norm(t, t.detach(), w, post_weight=w, gate=t.detach(), scale=w)
+    (dt,) = torch.autograd.grad((o2, r2), [t], (t.detach(), t.detach()))
+    assert torch.equal(out[-400:], o2) and torch.equal(res[-400:], r2) and torch.equal(dy[-400:], dt)
+
+
+@gpu
 def test_captured_replay_and_other_stream():
     v, cot = _inputs(300, 1024, torch.bfloat16)
     want = _run(v, "silu", cot)

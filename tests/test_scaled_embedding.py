@@ -164,6 +164,30 @@ def test_strides_shapes_and_repeatability():
 
 
 @gpu
+def test_offsets_over_32_bits():
+    """A table of 2.2e9 elements, and 2.2e9 elements looked up."""
+    V, N = 270007, 8192
+    w = torch.zeros(V, N, dtype=torch.bfloat16, device=DEV)
+    w[-50:] = torch.randn(50, N, device=DEV).to(torch.bfloat16)
+    ids = torch.randint(V - 50, V, (300,), generator=torch.Generator().manual_seed(0)).to(DEV)
+    assert w.numel() > 1 << 31
+    assert torch.equal(scaled_embedding(ids, w, 2.0), 2 * w[ids])
+    d = torch.randn(300, N, device=DEV).to(torch.bfloat16)
+    dw = scaled_embedding_backward(d, ids, V)
+    small = scaled_embedding_backward(d, ids - (V - 50), 50)
+    assert torch.equal(dw[-50:], small) and not bool(dw[:-50].any())
+    del dw
+    # ids of few rows, many tokens: the sums of the last tokens alone
+    d = torch.zeros(V, N, dtype=torch.bfloat16, device=DEV)
+    d[-30:] = 1
+    many = torch.arange(V, device=DEV) % 7
+    assert torch.equal(scaled_embedding(many, w[-7:], 1.0)[-20:], w[-7:][many[-20:]])
+    dw = scaled_embedding_backward(d, many, 7)
+    n = torch.bincount(many[-30:], minlength=7)
+    assert torch.equal(dw.float(), n[:, None].float().expand(7, N))
+
+
+@gpu
 def test_empty():
     w = torch.randn(10, 16, device=DEV, requires_grad=True)
     out = scaled_embedding(torch.empty(0, 3, dtype=torch.int64, device=DEV), w)
