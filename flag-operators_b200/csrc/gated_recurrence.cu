@@ -25,7 +25,8 @@
 // walked 64 steps at a time and every input is read once.  Where B * C gives too few CTAs to fill
 // the GPU, up to 8 CTAs of a cluster take consecutive tiles and exchange their maps through
 // distributed shared memory, as asynchronous stores that an mbarrier of the receiver counts (a cluster
-// barrier would wait for the outputs' stores too: 104 against TIME us at 1 x 16384 x 2048 bf16).  The next tiles' inputs are on their way
+// barrier waits for the outputs' stores too: backward 216 us with it, 192 us so, forward alike, at
+// 1 x 16384 x 2048 bf16).  The next tiles' inputs are on their way
 // meanwhile: a ring of kStages tiles in shared memory, each thread copying (cp.async) just the
 // elements that it will read, so that the ring needs no barrier.
 #include <type_traits>
@@ -225,20 +226,60 @@ __device__ __forceinline__ void send(void* to, const uint64_t* bar, uint32_t cta
 __device__ unsigned int g_glr_timeouts = 0;
 constexpr int kMaxPolls = 1 << 22;
 // Waits for phase `parity` of the mbarrier; gives up (and says so) after kMaxPolls polls.
-__device__ __forceinline__ bool wait_phase(const uint64_t* bar, uint32_t parity) {
+template <bool CLUSTER> __device__ __forceinline__ bool wait_phase(const uint64_t* bar, uint32_t parity) {
   for (int i = 0; i < kMaxPolls; ++i) {
     uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(shared_address(bar)), "r"(parity)
-        : "memory");
+    if (CLUSTER)
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(done)
+          : "r"(shared_address(bar)), "r"(parity)
+          : "memory");
+    else
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(done)
+          : "r"(shared_address(bar)), "r"(parity)
+          : "memory");
     if (done) return true;
   }
   return false;
 }
+
+// A chain of states through the warps of a CTA: warp w puts the state behind its steps of a round,
+// and its neighbour gets it.  Two places a warp, used in turn: a warp comes to round r + 2 only
+// with the state that its neighbour has put in round r + 1, behind its get of round r.
+template <typename F, int WARPS> struct Chain {
+  F state[2][WARPS][32];
+  uint64_t bar[2][WARPS];
+  bool dead;
+
+  __device__ __forceinline__ void init() {  // __syncthreads has to follow
+    if (threadIdx.x < 2 * WARPS)
+      asm volatile("mbarrier.init.shared.b64 [%0], 1;" ::"r"(shared_address(&bar[0][0] + threadIdx.x))
+                   : "memory");
+    if (threadIdx.x == 0) dead = false;
+  }
+  __device__ __forceinline__ void put(int64_t round, int w, F s) {
+    const int parity = (int)(round & 1), lane = threadIdx.x & 31;
+    state[parity][w][lane] = s;
+    __syncwarp();
+    if (lane == 0)
+      asm volatile("mbarrier.arrive.shared.b64 _, [%0];" ::"r"(shared_address(&bar[parity][w])) : "memory");
+  }
+  __device__ __forceinline__ F get(int64_t round, int w) {
+    const int parity = (int)(round & 1);
+    if (!dead && !wait_phase<false>(&bar[parity][w], (uint32_t)(round >> 1) & 1)) {
+      dead = true;  // no further waits: the kernel ends, its outputs are not complete
+      atomicAdd(&g_glr_timeouts, 1u);
+    }
+    return state[parity][w][threadIdx.x & 31];
+  }
+};
 
 // The maps of a round: of the CTA's warps, and (clusters) of the cluster's CTAs.  Two copies,
 // used in turn.  One of the CTA is written again only behind a barrier that every reader of it has
@@ -254,15 +295,13 @@ template <typename F, int WARPS, int CTAS> struct Maps {
   bool dead;
 
   __device__ __forceinline__ void init() {
-    if constexpr (CTAS > 1) {
-      if (threadIdx.x == 0) {
-        dead = false;
-        for (int k = 0; k < 2; ++k)
-          asm volatile("mbarrier.init.shared.b64 [%0], 1;" ::"r"(shared_address(&bar[k])) : "memory");
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-      }
-      cluster_barrier();
+    if (threadIdx.x == 0) {
+      dead = false;
+      for (int k = 0; k < 2; ++k)
+        asm volatile("mbarrier.init.shared.b64 [%0], 1;" ::"r"(shared_address(&bar[k])) : "memory");
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    cluster_barrier();
   }
 };
 
@@ -272,45 +311,36 @@ template <typename F, int WARPS, int CTAS> struct Maps {
 template <bool REVERSE, bool RESET, typename F, int WARPS, int CTAS>
 __device__ __forceinline__ F carry_in(Maps<F, WARPS, CTAS>& m, int64_t round, int w, F& S) {
   const int lane = threadIdx.x & 31, parity = (int)(round & 1);
+  const uint32_t n = cluster_size(), me = cluster_rank();
   F mine = S;
-  if constexpr (CTAS > 1) {
-    const uint32_t n = cluster_size(), me = cluster_rank();
-    if (threadIdx.x == 0)
-      asm volatile("mbarrier.arrive.expect_tx.shared.b64 _, [%0], %1;" ::"r"(shared_address(&m.bar[parity])),
-                   "r"(n * 32 * (uint32_t)sizeof(typename Maps<F, WARPS, CTAS>::Both))
-                   : "memory");
-    if (w < (int)n) {  // warp w hands the CTA's map to CTA w
-      F a = all_<F>(1.f), h = all_<F>(0.f);
+  if (threadIdx.x == 0)
+    asm volatile("mbarrier.arrive.expect_tx.shared.b64 _, [%0], %1;" ::"r"(shared_address(&m.bar[parity])),
+                 "r"(n * 32 * (uint32_t)sizeof(typename Maps<F, WARPS, CTAS>::Both))
+                 : "memory");
+  if (w < (int)n) {  // warp w hands the CTA's map to CTA w
+    F a = all_<F>(1.f), h = all_<F>(0.f);
 #pragma unroll
-      for (int k = 0; k < WARPS; ++k) {
-        const int q = REVERSE ? WARPS - 1 - k : k;
-        const F ak = m.A[parity][q][lane];
-        h = through<RESET>(h, ak, m.H[parity][q][lane]);
-        a = finite(mul_(a, ak));
-      }
-      send(&m.cta[parity][me][lane], &m.bar[parity], w, a, h);
-    }
-    if (!m.dead && !wait_phase(&m.bar[parity], (uint32_t)(round >> 1) & 1)) {
-      m.dead = true;  // no further waits: the kernel ends, its outputs are not complete
-      atomicAdd(&g_glr_timeouts, 1u);
-    }
-    for (uint32_t k = 0; k < n; ++k) {
-      const uint32_t q = REVERSE ? n - 1 - k : k;
-      if (q == me) mine = S;
-      S = through<RESET>(S, m.cta[parity][q][lane].A, m.cta[parity][q][lane].H);
-    }
-#pragma unroll
-    for (int k = 0; k < WARPS - 1; ++k) {
-      const int q = REVERSE ? WARPS - 1 - k : k;
-      if (REVERSE ? q > w : q < w) mine = through<RESET>(mine, m.A[parity][q][lane], m.H[parity][q][lane]);
-    }
-  } else {
-#pragma unroll 4  // more would hold the maps of all warps in registers at once
     for (int k = 0; k < WARPS; ++k) {
       const int q = REVERSE ? WARPS - 1 - k : k;
-      if (q == w) mine = S;
-      S = through<RESET>(S, m.A[parity][q][lane], m.H[parity][q][lane]);
+      const F ak = m.A[parity][q][lane];
+      h = through<RESET>(h, ak, m.H[parity][q][lane]);
+      a = finite(mul_(a, ak));
     }
+    send(&m.cta[parity][me][lane], &m.bar[parity], w, a, h);
+  }
+  if (!m.dead && !wait_phase<true>(&m.bar[parity], (uint32_t)(round >> 1) & 1)) {
+    m.dead = true;  // no further waits: the kernel ends, its outputs are not complete
+    atomicAdd(&g_glr_timeouts, 1u);
+  }
+  for (uint32_t k = 0; k < n; ++k) {
+    const uint32_t q = REVERSE ? n - 1 - k : k;
+    if (q == me) mine = S;
+    S = through<RESET>(S, m.cta[parity][q][lane].A, m.cta[parity][q][lane].H);
+  }
+#pragma unroll
+  for (int k = 0; k < WARPS - 1; ++k) {
+    const int q = REVERSE ? WARPS - 1 - k : k;
+    if (REVERSE ? q > w : q < w) mine = through<RESET>(mine, m.A[parity][q][lane], m.H[parity][q][lane]);
   }
   return mine;
 }
@@ -366,8 +396,9 @@ glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
   constexpr int N = kFwdSteps;
   extern __shared__ __align__(16) uint8_t smem[];
   auto& ring = *reinterpret_cast<FwdRing<T, G, V>*>(smem);
-  __shared__ Maps<F, kFwdWarps, CTAS> maps;
-  maps.init();
+  __shared__ std::conditional_t<(CTAS > 1), Maps<F, kFwdWarps, CTAS>, Chain<F, kFwdWarps>> link;
+  link.init();
+  __syncthreads();
   const Place p = place<V, (CTAS > 1)>(C);
   const int lane = threadIdx.x & 31, w = warp_index();
   const int64_t tiles = (L + kFwdTile - 1) / kFwdTile, rounds = (tiles + p.size - 1) / p.size;
@@ -448,11 +479,17 @@ glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
       A = mul_(A, a[i]);
       H = fma_(a[i], H, b[i]);
     }
-    const int parity = (int)(round & 1);
-    maps.A[parity][w][lane] = finite(A);
-    maps.H[parity][w][lane] = H;
-    __syncthreads();
-    F hv = carry_in<false, RESET>(maps, round, w, S);
+    A = finite(A);
+    F hv = S;  // the state in front of the warp's steps
+    if constexpr (CTAS > 1) {
+      link.A[round & 1][w][lane] = A;
+      link.H[round & 1][w][lane] = H;
+      __syncthreads();
+      hv = carry_in<false, RESET>(link, round, w, S);
+    } else {
+      if (round > 0 || w > 0) hv = link.get(w ? round : round - 1, w ? w - 1 : kFwdWarps - 1);
+      link.put(round, w, through<RESET>(hv, A, H));
+    }
     if (p.on) {
       if (ckpt && n > 0 && t0 % FO_GLR_CHECKPOINT == 0)
         Elem<float, V>::store(ckpt + (p.b * checkpoints + t0 / FO_GLR_CHECKPOINT) * C + p.c, hv);
@@ -530,9 +567,12 @@ glr_bwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
   constexpr int N = kBwdSteps, WARPS = kBwdWarps;
   extern __shared__ __align__(16) uint8_t smem[];
   auto& ring = *reinterpret_cast<BwdRing<T, G, V>*>(smem);
-  __shared__ Maps<F, WARPS, CTAS> maps;  // of R -> A R + Q
-  __shared__ F map_h[2][WARPS][32];      // of s -> A s + H
-  maps.init();
+  // links of the a_t D_t of the steps behind (R -> A R + Q), and of the states in front (s -> A s + H)
+  __shared__ std::conditional_t<(CTAS > 1), Maps<F, WARPS, CTAS>, Chain<F, WARPS>> link;
+  __shared__ std::conditional_t<(CTAS > 1), F[2][WARPS][32], Chain<F, WARPS>> link_h;
+  link.init();
+  if constexpr (CTAS == 1) link_h.init();
+  __syncthreads();
   const Place p = place<V, (CTAS > 1)>(C);
   const int lane = threadIdx.x & 31, w = warp_index();
   const int64_t tiles = (L + kBwdTile - 1) / kBwdTile, rounds = (tiles + p.size - 1) / p.size;
@@ -629,14 +669,33 @@ glr_bwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
       if (i + 1 < N) Q = RESET && (rs >> (i + 1) & 1) ? d_of(i) : fma_(a[i + 1], Q, d_of(i));
       else Q = d_of(i);
     }
-    maps.A[parity][w][lane] = finite(A);
-    maps.H[parity][w][lane] = RESET && (rs & 1) ? all_<F>(0.f) : mul_(a[0], Q);
-    map_h[parity][w][lane] = H;
-    __syncthreads();
-    F d = carry_in<true, RESET>(maps, k, w, R);
+    A = finite(A);
+    Q = RESET && (rs & 1) ? all_<F>(0.f) : mul_(a[0], Q);
+    F d = R;  // a_t D_t of the step behind the warp's
+    if constexpr (CTAS > 1) {
+      link.A[parity][w][lane] = A;
+      link.H[parity][w][lane] = Q;
+      link_h[parity][w][lane] = H;
+      __syncthreads();
+      d = carry_in<true, RESET>(link, k, w, R);
 #pragma unroll 4
-    for (int q = 0; q < WARPS - 1; ++q)
-      if (q < w) hv = through<RESET>(hv, maps.A[parity][q][lane], map_h[parity][q][lane]);
+      for (int q = 0; q < WARPS - 1; ++q)
+        if (q < w) hv = through<RESET>(hv, link.A[parity][q][lane], link_h[parity][q][lane]);
+    } else {
+      auto from_front = [&] {
+        if (w > 0) hv = link_h.get(k, w - 1);
+        if (w + 1 < WARPS) link_h.put(k, w, through<RESET>(hv, A, H));
+      };
+      auto from_behind = [&] {
+        if (k > 0 || w + 1 < WARPS) d = link.get(w + 1 < WARPS ? k : k - 1, w + 1 < WARPS ? w + 1 : 0);
+        R = through<RESET>(d, A, Q);
+        link.put(k, w, R);
+      };
+      // the end of the tile that is nearer comes first
+      if (w < WARPS / 2) from_front();
+      from_behind();
+      if (w >= WARPS / 2) from_front();
+    }
     if (p.on) {
       F D[N];
 #pragma unroll
@@ -686,13 +745,14 @@ glr_bwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
   copy_wait<0>();
   if (dh0 && p.on && p.rank == 0 && w == 0) Elem<float, V>::store(dh0 + p.b * C + p.c, R);
   if (LOGITS && ddecay_part) {
+    auto& sums = ring.mi;  // of no use any more
     __syncthreads();
-    map_h[0][w][lane] = sum;
+    sums[w][0][lane] = sum;
     __syncthreads();
     if (w == 0 && p.on) {
-      F t = map_h[0][0][lane];
+      F t = sums[0][0][lane];
 #pragma unroll
-      for (int k = 1; k < WARPS; ++k) t = add_(t, map_h[0][k][lane]);
+      for (int k = 1; k < WARPS; ++k) t = add_(t, sums[k][0][lane]);
       Elem<float, V>::store(ddecay_part + (p.b * p.size + p.rank) * C + p.c, t);
     }
   }
