@@ -31,6 +31,7 @@
 // elements that it will read, so that the ring needs no barrier.
 #include <type_traits>
 
+#include "cluster.cuh"
 #include "gates.cuh"
 
 namespace fo {
@@ -185,30 +186,8 @@ template <int N> __device__ __forceinline__ void copy_wait() {
 }
 
 // ---------------------------------------------------------------------------
-// Clusters
+// Links between warps and between the CTAs of a cluster
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
-                   : "memory");
-}
-__device__ __forceinline__ uint32_t shared_address(const void* p) {
-  return (uint32_t)__cvta_generic_to_shared(p);
-}
-__device__ __forceinline__ uint32_t remote_address(const void* p, uint32_t cta) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(shared_address(p)), "r"(cta));
-  return r;
-}
 // Two values into CTA `cta`'s copy of `to`, counted by its copy of `bar`
 __device__ __forceinline__ void send(void* to, const uint64_t* bar, uint32_t cta, float a, float h) {
   asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(

@@ -26,6 +26,7 @@
 // through L1 and L2.
 #include <type_traits>
 
+#include "cluster.cuh"
 #include "gates.cuh"
 
 namespace fo {
@@ -91,8 +92,9 @@ struct Columns<T, W, TPR, VPT, true, S> {
   static constexpr int kRingBytes = 2 * S * VPT * kThreads * 16;
   uint4* ring;
   int v0, nvec;
-  __device__ __forceinline__ Columns(uint8_t* smem, int64_t N)
-      : ring(reinterpret_cast<uint4*>(smem) + threadIdx.x), v0(threadIdx.x % TPR), nvec((int)(N / E)) {}
+  // n: the elements of the row (or of the CTA's part of it)
+  __device__ __forceinline__ Columns(uint8_t* smem, int64_t n)
+      : ring(reinterpret_cast<uint4*>(smem) + threadIdx.x), v0(threadIdx.x % TPR), nvec((int)(n / E)) {}
   __device__ __forceinline__ uint4* slot(int stage, int k, int i) {
     return ring + ((stage * S + k) * VPT + i) * kThreads;
   }
@@ -204,21 +206,31 @@ struct Columns<T, W, TPR, VPT, false, S> {
   }
 };
 
-// Sums of K values over the TPR threads of a row, in every one of them.  `red`: [K][warps], not
-// used by the reduction before this one.
-template <int TPR, int K>
+// Sums of K values over the TPR threads of a row (of CTAS CTAs each), in every one of them.  `red`:
+// [K][warps], not used by the reduction before this one.
+template <int TPR, int CTAS = 1, int K>
 __device__ __forceinline__ void row_sum(float (&v)[K], float (*red)[32]) {
+  constexpr int kWarps = (TPR + 31) / 32 * CTAS;
+  static_assert(kWarps <= 32, "a lane for each warp of the row");
 #pragma unroll
   for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1)
 #pragma unroll
     for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
-  if constexpr (TPR > 32) {
-    constexpr int kWarps = TPR / 32;
+  if constexpr (kWarps > 1) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    if (lane == 0)
+    if constexpr (CTAS > 1) {
+      const int at = (int)cluster_rank() * (TPR / 32) + w;
+      if (lane < CTAS)
 #pragma unroll
-      for (int k = 0; k < K; ++k) red[k][w] = v[k];
-    __syncthreads();
+        for (int k = 0; k < K; ++k) store_remote(&red[k][at], lane, v[k]);
+      __syncwarp();
+      cluster_barrier();
+    } else {
+      if (lane == 0)
+#pragma unroll
+        for (int k = 0; k < K; ++k) red[k][w] = v[k];
+      __syncthreads();
+    }
 #pragma unroll
     for (int k = 0; k < K; ++k) v[k] = red[k][lane % kWarps];
 #pragma unroll
@@ -355,7 +367,8 @@ rrn_fwd_kernel(Fwd a) {
   }
 }
 
-template <typename T, typename W, int TPR, int VPT, bool WIDE>
+// CTAS > 1: a row is split over the CTAs of a cluster, a multiple of 16 bytes each.
+template <typename T, typename W, int TPR, int VPT, bool WIDE, int CTAS>
 __global__ void __launch_bounds__(Shape<TPR>::kThreads, 512 / Shape<TPR>::kThreads)
 rrn_bwd_kernel(Bwd a) {
   using S = Shape<TPR>;
@@ -364,24 +377,30 @@ rrn_bwd_kernel(Bwd a) {
   constexpr int P = C::P;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float red[6][32];
-  const int N = (int)a.N;
+  // the CTA's columns: N from c0 on
+  const int share = CTAS > 1 ? (int)((a.N / C::E + CTAS - 1) / CTAS) * C::E : (int)a.N;
+  const int c0 = CTAS > 1 ? (int)cluster_rank() * share : 0;
+  const int N = a.N - c0 < share ? (int)(a.N - c0) : share;
   // w and s w_post in fp32, in front of the ring
   float *sw = reinterpret_cast<float*>(smem), *ssw = sw + (N + 3) / 4 * 4;
   C col(smem + weight_bytes(N), N);
   for (int j = threadIdx.x; j < N; j += S::kThreads) {
-    sw[j] = to_f<W>(((const W*)a.w)[j]);
-    ssw[j] = (a.sv ? to_f<W>(((const W*)a.sv)[j]) : a.s) * (a.wp ? to_f<W>(((const W*)a.wp)[j]) : 1.f);
+    sw[j] = to_f<W>(((const W*)a.w)[c0 + j]);
+    ssw[j] = (a.sv ? to_f<W>(((const W*)a.sv)[c0 + j]) : a.s) *
+             (a.wp ? to_f<W>(((const W*)a.wp)[c0 + j]) : 1.f);
   }
   __syncthreads();
-  const int64_t step = (int64_t)gridDim.x * S::kRows, mine = threadIdx.x / TPR;
-  int64_t base = (int64_t)blockIdx.x * S::kRows;
-  const int64_t z = sizeof(T), r0 = base + mine;
-  const uint8_t *py = (const uint8_t*)a.y + r0 * a.y_ld * z + col.first(),
-                *pr = (const uint8_t*)a.r + r0 * a.r_ld * z + col.first(),
-                *pg = (const uint8_t*)a.gate + r0 * a.g_ld * z + col.first();
+  if constexpr (CTAS > 1) cluster_barrier();  // every CTA runs before its memory is written to
+  const int64_t groups = gridDim.x / CTAS, group = blockIdx.x / CTAS;
+  const int64_t step = groups * S::kRows, mine = threadIdx.x / TPR;
+  int64_t base = group * S::kRows;
+  const int64_t z = sizeof(T), r0 = base + mine, first = c0 * z + col.first();
+  const uint8_t *py = (const uint8_t*)a.y + r0 * a.y_ld * z + first,
+                *pr = (const uint8_t*)a.r + r0 * a.r_ld * z + first,
+                *pg = (const uint8_t*)a.gate + r0 * a.g_ld * z + first;
   const int64_t sy = step * a.y_ld * z, sr = step * a.r_ld * z, sg = step * a.g_ld * z,
                 sn = step * a.N * z;
-  int64_t to = r0 * a.N * z + col.first();
+  int64_t to = r0 * a.N * z + first;
   // ahead: the row is `ahead` bytes behind the one at `to`
   auto fetch = [&](int64_t row, int stage, int64_t ahead) {
     if (row < a.M) {
@@ -398,7 +417,7 @@ rrn_bwd_kernel(Bwd a) {
   // What is absent is filled in, so that the arithmetic has no branches: a gate with 100 (its
   // sigmoid is 1), gradients with 0.
   const bool silu = a.act == FO_ACT_SILU;
-  const float rn = 1.f / (float)N;
+  const float rn = 1.f / (float)a.N;
   struct Part {
     Raw y, r, z, d, dr;
   };
@@ -462,7 +481,7 @@ rrn_bwd_kernel(Bwd a) {
       }
     }
     float sum[3] = {s1.x + s1.y, s2.x + s2.y, s3.x + s3.y};
-    row_sum<TPR>(sum, red + 3 * s);
+    row_sum<TPR, CTAS>(sum, red + 3 * s);
     const float c2 = inv2 * inv2 * inv2 * (sum[0] * rn);
     const float c1 = a.wp ? inv1 * inv1 * inv1 * (fmaf(-c2, sum[2], sum[1]) * rn) : 0.f;
     const float2 m2 = all_<float2>(-c2), m1 = all_<float2>(-c1);
@@ -496,9 +515,9 @@ rrn_bwd_kernel(Bwd a) {
       }
     }
   }
-  // part[2][gridDim.x][N]; rows side by side in the CTA are added up first
-  const int64_t stride = (int64_t)gridDim.x * a.N;
-  float* part = a.part + (int64_t)blockIdx.x * a.N;
+  // part[2][groups][N]; rows side by side in the CTA are added up first
+  const int64_t stride = groups * a.N;
+  float* part = a.part + group * a.N + c0;
   if constexpr (S::kRows == 1) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
@@ -523,6 +542,7 @@ rrn_bwd_kernel(Bwd a) {
       part[j / N * stride + j % N] = t;
     }
   }
+  if constexpr (CTAS > 1) cluster_barrier();  // none leaves while another writes to it
 }
 
 // ---------------------------------------------------------------------------
@@ -694,8 +714,8 @@ int64_t partial_rows(int64_t M, int64_t N) {
 }
 
 // Calls f(TPR, VPT, WIDE) with the smallest shape whose threads cover a row of N elements: a warp or
-// less for the narrowest rows (no barrier), else a CTA of up to 512 threads.  Returns -1 where
-// none does.
+// less for the narrowest rows (no barrier), else a CTA of up to 512 threads, and 1024 for
+// the widest (the forward's; backward two CTAs of 512 share such a row).  Returns -1 where none does.
 template <typename T, typename F> int with_shape(bool wide, int64_t N, F&& f) {
   using std::integral_constant;
   auto go = [&](auto tpr, auto vpt, auto w) {
@@ -712,6 +732,7 @@ template <typename T, typename F> int with_shape(bool wide, int64_t N, F&& f) {
     FO_SHAPE(256, 1, E, std::true_type);
     FO_SHAPE(512, 1, E, std::true_type);
     FO_SHAPE(512, 2, E, std::true_type);
+    FO_SHAPE(1024, 2, E, std::true_type);
   } else {
     FO_SHAPE(32, 1, 2, std::false_type);
     FO_SHAPE(32, 2, 2, std::false_type);
@@ -736,7 +757,7 @@ bool wide_ok(int64_t N, const void* const* rows, const int64_t* lds, int n,
 
 template <typename K, typename A>
 int launch(const char* what, K kernel, int64_t ctas, int threads, int smem, const A& a,
-           cudaStream_t st) {
+           cudaStream_t st, int cluster = 1) {
   if (smem > 40 * 1024) {
     cudaError_t e = allow_shared((const void*)kernel, 227 * 1024 - 1024);
     if (e != cudaSuccess) {
@@ -745,7 +766,26 @@ int launch(const char* what, K kernel, int64_t ctas, int threads, int smem, cons
       return FO_ECUDA;
     }
   }
-  kernel<<<(unsigned)ctas, threads, smem, st>>>(a);
+  if (cluster == 1) {
+    kernel<<<(unsigned)ctas, threads, smem, st>>>(a);
+    return check_launch(what);
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(ctas * cluster));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = cluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a)) {
+    cudaGetLastError();
+    set_error("%s: %s", what, cudaGetErrorString(e));
+    return FO_ECUDA;
+  }
   return check_launch(what);
 }
 
@@ -780,15 +820,19 @@ int run_bwd(const Bwd& a, cudaStream_t st) {
   int G = 0;
   int rc = with_shape<T>(wide_ok<T>(a.N, rows, lds, 8, vs, 3), a.N, [&](auto tpr, auto vpt, auto wide) {
     using S = Shape<tpr>;
-    const int ring = Columns<T, W, tpr, vpt, wide, 5>::kRingBytes + weight_bytes(a.N);
-    const int sums = S::kRows > 1 ? (int)(S::kRows * 2 * a.N * 4) : 0;
+    constexpr int kCtas = tpr > 512 ? 2 : 1, kTpr = tpr / kCtas;  // of a row
+    using Half = Shape<kTpr>;
+    const int64_t columns = (a.N + kCtas - 1) / kCtas + (kCtas > 1 ? Vec16<T>::E : 0);
+    const int ring = Columns<T, W, kTpr, vpt, wide, 5>::kRingBytes + weight_bytes(columns);
+    const int sums = Half::kRows > 1 ? (int)(Half::kRows * 2 * a.N * 4) : 0;
     const int smem = ring > sums ? ring : sums;
-    int64_t ctas = num_sms() * resident(512, S::kThreads, smem);
-    const int64_t need = (a.M + S::kRows - 1) / S::kRows, most = partial_rows(a.M, a.N);
+    int64_t ctas = num_sms() / kCtas * resident(512, Half::kThreads, smem);
+    const int64_t need = (a.M + Half::kRows - 1) / Half::kRows, most = partial_rows(a.M, a.N);
     if (ctas > need) ctas = need;
     if (ctas > most) ctas = most;
     G = (int)ctas;
-    return launch("rrn_bwd_kernel", rrn_bwd_kernel<T, W, tpr, vpt, wide>, ctas, S::kThreads, smem, a, st);
+    return launch("rrn_bwd_kernel", rrn_bwd_kernel<T, W, kTpr, vpt, wide, kCtas>, ctas, Half::kThreads,
+                  smem, a, st, kCtas);
   });
   if (rc == -1) {
     rrn_bwd_generic_kernel<T, W><<<row_grid(a.M), 256, 0, st>>>(a);
