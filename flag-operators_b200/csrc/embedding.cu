@@ -19,6 +19,13 @@
 //     runs of 16 pieces of one id, so that no chain is long).
 // Most rows of dW have no token and are zeros: spare CTAs of the kernels 1 and 2, which leave the
 // memory idle, write all of dW as zeros meanwhile.
+//
+// Measured (B200, 16384 tokens distributed as words, 128256 x 4096 bf16): lookup 30 us (268 MB less
+// what repeats); gradient 127 us sort (with 788 MB of zeros), 48 us merge (with 262 MB), 33 us
+// pieces, 4 us runs, 11 us join, which is 1.25 GB at 5.6 TB/s.  Finding each row's tokens in the
+// kernel that writes dW was slower (241 us for that kernel alone: its CTAs wait for bounds,
+// positions and rows one after the other).  30011 tokens, a third of them one id, 5003 x 771 fp32:
+// 27 us and 74 us; there the bisections and the unaligned rows' 4-byte accesses count.
 #include <type_traits>
 
 #include "common.cuh"
@@ -534,8 +541,8 @@ extern "C" int fo_embedding_fwd(const void* ids, const void* weight, void* out, 
   return with_types(dtype, index_dtype, [&](auto t, auto i) {
     using E = decltype(t);
     using I = decltype(i);
-    // Four rows a CTA, where that leaves enough CTAs: 41 us with one, 37 us with four for 30011 rows
-    // of 771 fp32 elements.
+    // Four rows a CTA, where that leaves enough CTAs: 41 us with one, 37 with four for 30011 rows of
+    // 771 fp32 elements.
     const bool four = T >= 16 * (int64_t)num_sms();
     auto run = [&](auto wide) {
       constexpr int K = wide ? 2 : 4;

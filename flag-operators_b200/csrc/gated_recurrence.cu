@@ -17,18 +17,28 @@
 // backward reads anyway, and gradients do not see the output's rounding to 16 bits.
 // All of it is held in fp32; h and the gradients are rounded once when they are written.
 //
-// Split.  Time is cut into tiles of 64 steps, channels into slabs of 32 lanes (two channels a lane
-// where C, the strides and the addresses allow it, so a warp's row is one 128-byte line in 16
-// bits).  A CTA's 8 warps take 8 consecutive steps of a tile each, held in registers: over its
-// steps a warp is the map s -> A s + H (backward: R -> A R + Q), the 8 maps meet in shared memory,
-// and each warp then walks its steps once from the state that enters them.  So the axis is
-// walked 64 steps at a time and every input is read once.  Where B * C gives too few CTAs to fill
-// the GPU, up to 8 CTAs of a cluster take consecutive tiles and exchange their maps through
-// distributed shared memory, as asynchronous stores that an mbarrier of the receiver counts (a cluster
-// barrier waits for the outputs' stores too: backward 216 us with it, 192 us so, forward alike, at
-// 1 x 16384 x 2048 bf16).  The next tiles' inputs are on their way
-// meanwhile: a ring of kStages tiles in shared memory, each thread copying (cp.async) just the
-// elements that it will read, so that the ring needs no barrier.
+// Split.  Channels are cut into slabs of 32 lanes (two channels a lane with 16-bit gates where C, the
+// strides and the addresses allow it, so that a warp's row is a 128-byte line), time into rounds.
+// In a round each of a CTA's 8 warps takes 16 (backward: 8) consecutive steps, whose gates it
+// computes independently of any state; over them it is a map s -> A s + H (backward: R -> A R + Q),
+// and it walks them once, from the state that enters them.  That state comes
+//  - where slabs * B give every SM a CTA: from the neighbouring warp, as a chain through shared memory
+//    (an mbarrier a link), so that warps run ahead of one another and the gates of one overlap the
+//    walk of another: 235 us against 266 us with a barrier for all warps, forward at 8 x 8192 x 2048
+//    bf16 logits;
+//  - with fewer slabs: up to 8 CTAs of a cluster take consecutive tiles, each warp's map is put
+//    together with those in front of it, and the CTAs exchange theirs as asynchronous stores that an
+//    mbarrier of the receiver counts (a cluster barrier waits for the outputs' stores too: backward
+//    216 us with it, 192 us so, at 1 x 16384 x 2048 bf16).
+// Inputs come through a ring of two rounds in shared memory (cp.async), which each warp fills and reads
+// by itself.  Every input is read once and every output written once.
+//
+// What bounds it (1 x B200, bf16): gates as values run at the memory's rate (forward 160 us at
+// 8 x 8192 x 2048, 1.07 GB).  With logits an element takes five exponentials, reciprocals and roots,
+// which alone take 150 us there: 235 us forward (floor 164).  Backward 500 us (floor 287): 154
+// instructions for a pair of channels at 57 % of the issue rate, 16 warps on an SM (its shared
+// memory is full).  Both lose an eighth to 256 CTAs on 148 SMs.
+
 #include <type_traits>
 
 #include "cluster.cuh"
@@ -37,7 +47,10 @@
 namespace fo {
 namespace {
 
-constexpr int kFwdSteps = 16, kFwdWarps = 8;  // steps of a thread in a round, and warps of a CTA
+// Steps of a thread in a round, and warps of a CTA.  Forward at 8 x 8192 x 2048 bf16: 235 us; with
+// 8 steps and 16 warps 239, 8 and 8 267, 16 and 12 263, 4 and 16 288.  Backward needs the registers
+// for 8 steps.
+constexpr int kFwdSteps = 16, kFwdWarps = 8;
 constexpr int kFwdTile = kFwdSteps * kFwdWarps;
 constexpr int kBwdSteps = 8, kBwdWarps = 8;
 constexpr int kBwdTile = kBwdSteps * kBwdWarps;

@@ -14,16 +14,23 @@
 //   sum k y = sum q y (dr' + inv2 e) - c2 sum q y r',  q = s act w_post, c2 = inv2^3 mean(e r')
 // gets all three sums of a row from one pass and one block reduction.
 //
-// Both are bound by memory.  Where rows are 16-byte aligned and fit, TPR threads own a row, VPT
-// 16-byte vectors each, and CTAs walk over the rows: every input is read once, by cp.async into a
-// ring of two rows in shared memory (the next row is on its way while this one is reduced and
-// written), and a thread only ever reads the slots that it filled, so the ring needs no barrier.
+// Both are bound by memory.  TPR threads own a row, VPT 16-byte vectors each, and CTAs walk over the
+// rows: every input is read once, by cp.async into a ring of two rows in shared memory (the next row
+// is on its way while this one is reduced and written), and a thread only ever reads the slots that
+// it filled, so the ring needs no barrier.  Rows that 16-byte vectors do not fit are read into
+// registers instead; rows wider than 1024 vectors take 1024 threads, backward two CTAs of a cluster
+// that add their sums up through distributed shared memory; still wider ones the generic kernels
+// (several passes over the row, through L1 and L2).
 // The backward keeps its threads' column sums (of dw and A) in registers over all rows of the CTA,
 // writes them as one partial row a CTA, and a column kernel adds those up in their order; s w_post
-// and w are kept in shared memory in fp32.  Its arithmetic is what limits it next (a sigmoid and some
-// thirty operations an element), so it is done on pairs.  Rows that 16-byte vectors do not fit are
-// read into registers instead; wider rows take the generic kernels: several passes over the row,
-// through L1 and L2.
+// and w are kept in shared memory in fp32.
+//
+// Measured (B200): 16384 x 8192 bf16 with gate and both norms 237 us forward (5 streams, 1.34 GB,
+// 5.7 TB/s) and 430 us backward (8 streams, 5.0 TB/s; 62 instructions an element at half the issue
+// rate, one CTA of 512 threads on an SM); 4096 x 4096 fp32 48 and 62 us; 4096 x 16384 bf16 150 and
+// 265 us.  1024 threads with one vector each were slower (297 us forward), and so was the backward
+// with 64 registers (740 us: it spills).
+
 #include <type_traits>
 
 #include "cluster.cuh"

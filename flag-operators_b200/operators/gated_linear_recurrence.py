@@ -20,6 +20,8 @@ else is copied.  h has x's dtype; states are fp32 [B, C].
   reset           bool [B, L]: steps that start again from nothing (a_t = 0), for packed sequences
   output_final_state   also return the state after the last token
 
+Gates above 1 make the state grow; their product over any 128 consecutive steps has to stay
+within the fp32 range (over an empty state it may leave it).
 A padded step that keeps the state (g = 1, beta = 0 as values; g = -inf as logits) must hold
 a finite x.  The state is fp32 throughout and h is rounded once.
 
