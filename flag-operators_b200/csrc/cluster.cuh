@@ -19,6 +19,11 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
                    : "memory");
 }
+// As cluster_barrier, but orders no memory: does not wait for stores on their way.
+__device__ __forceinline__ void cluster_meet() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
 __device__ __forceinline__ uint32_t shared_address(const void* p) {
   return (uint32_t)__cvta_generic_to_shared(p);
 }

@@ -35,8 +35,8 @@
 //
 // What bounds it (1 x B200, bf16): gates as values run at the memory's rate (forward 160 us at
 // 8 x 8192 x 2048, 1.07 GB).  With logits an element takes five exponentials, reciprocals and roots,
-// which alone take 150 us there: 235 us forward (floor 164).  Backward 500 us (floor 287): 154
-// instructions for a pair of channels at 57 % of the issue rate, 16 warps on an SM (its shared
+// which alone take 150 us there: 235 us forward (floor 164).  Backward 500 us (floor 287): 140
+// instructions for a pair of channels at 55 % of the issue rate, 16 warps on an SM (its shared
 // memory is full).  Both lose an eighth to 256 CTAs on 148 SMs.
 
 #include <type_traits>
@@ -503,6 +503,7 @@ glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
   }
   if (L == 0 && hT && p.on && w == 0) Elem<float, V>::store(hT + p.b * C + p.c, S);
   copy_wait<0>();
+  if constexpr (CTAS > 1) cluster_meet();  // none leaves while another may send to it
 }
 
 // ---------------------------------------------------------------------------
@@ -748,6 +749,7 @@ glr_bwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
       Elem<float, V>::store(ddecay_part + (p.b * p.size + p.rank) * C + p.c, t);
     }
   }
+  if constexpr (CTAS > 1) cluster_meet();  // none leaves while another may send to it
 }
 
 // ddecay[c] = sigmoid(decay) / softplus(decay) * the sum of the partial rows of du u, in their
