@@ -10,7 +10,7 @@ Without `decay` the gates are values, as in chunk_gated_delta_rule: a_t = g_t,
 b_t = beta_t x_t.  With `decay` ([C]) they are logits, and the input is scaled so
 that the state keeps its variance:
     a_t = exp(-decay_scale softplus(decay) sigmoid(g_t))
-    b_t = sqrt(1 - a_t^2) sigmoid(beta_t) x_t
+    b_t = sqrt(1 - a_t^2) sigmoid(beta_t) x_t      (decay_scale finite, not negative)
 
 x: [B, L, C] fp32 / fp16 / bf16; g, beta: [B, L, C] of x's dtype or both fp32 (gates that are
 values near 1 need fp32: bf16 has no number between 0.996 and 1).  x, g and beta may be
@@ -28,12 +28,15 @@ a finite x.  The state is fp32 throughout and h is rounded once.
 All of x, g, beta, decay and initial_state are differentiable, once (csrc/gated_recurrence.cu;
 the backward reads x, g, beta and dh and recomputes the states from fp32 checkpoints every
 64 steps).  gated_linear_recurrence_step is for decoding: x, g, beta [B, C], `state` [B, C] fp32
-is overwritten, and nothing is differentiated.
+is overwritten (it must not share memory with the other arguments), and nothing is differentiated.
+With `reset`, a NaN or infinity in the state in front of a run of gates whose product is 0 may not
+reach the steps behind it.
 """
 from __future__ import annotations
 
 import ctypes
 import logging
+import math
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -45,7 +48,7 @@ logger = logging.getLogger(__name__)
 CHECKPOINT = 64  # FO_GLR_CHECKPOINT of include/flagops.h
 
 
-def _check_gates(op, x, g, beta, decay):
+def _check_gates(op, x, g, beta, decay, scale):
     if g.shape != x.shape or beta.shape != x.shape:
         raise ValueError(f"{op}: g shape {tuple(g.shape)} and beta shape {tuple(beta.shape)} must be "
                          f"x's {tuple(x.shape)}")
@@ -56,6 +59,8 @@ def _check_gates(op, x, g, beta, decay):
         raise TypeError(f"{op}: dtype {x.dtype} is not supported")
     if decay is not None and decay.shape != x.shape[-1:]:
         raise ValueError(f"{op}: decay shape {tuple(decay.shape)}, expected ({x.shape[-1]},)")
+    if not (math.isfinite(scale) and scale >= 0):  # a gate above 1 has no root of 1 - a^2
+        raise ValueError(f"{op}: decay_scale must be finite and not negative, got {scale}")
     dev = x.device
     if g.device != dev or beta.device != dev or (decay is not None and decay.device != dev):
         raise ValueError(f"{op}: g, beta and decay must be on the same device as x")
@@ -151,7 +156,8 @@ def gated_linear_recurrence(
     _lib.require_cuda(x, op)
     if x.dim() != 3:
         raise ValueError(f"{op}: x must be [B, L, C], got shape {tuple(x.shape)}")
-    _check_gates(op, x, g, beta, decay)
+    scale = float(decay_scale)
+    _check_gates(op, x, g, beta, decay, scale)
     B, L, C = x.shape
     h0 = initial_state
     if h0 is not None:
@@ -168,7 +174,6 @@ def gated_linear_recurrence(
     if decay is not None:
         decay = decay.to(torch.float32).contiguous()
     x, g, beta = _rows(x), _rows(g), _rows(beta)
-    scale = float(decay_scale)
     if torch.is_grad_enabled() and (x.requires_grad or g.requires_grad or beta.requires_grad
                                     or (decay is not None and decay.requires_grad)
                                     or (h0 is not None and h0.requires_grad)):
@@ -192,7 +197,8 @@ def gated_linear_recurrence_step(
     _lib.require_cuda(x, op)
     if x.dim() != 2:
         raise ValueError(f"{op}: x must be [B, C], got shape {tuple(x.shape)}")
-    _check_gates(op, x, g, beta, decay)
+    scale = float(decay_scale)
+    _check_gates(op, x, g, beta, decay, scale)
     if state.shape != x.shape or state.dtype != torch.float32 or state.device != x.device \
             or not state.is_contiguous():
         raise ValueError(f"{op}: state must be a contiguous float32 tensor of shape {tuple(x.shape)} on "
@@ -209,8 +215,10 @@ def gated_linear_recurrence_step(
     h = x.new_empty((B, C))
     with _lib.on_device(x):
         _lib.call("fo_glr_step", _lib.ptr(x), _lib.ptr(g), _lib.ptr(beta), _lib.ptr(decay),
-                  _lib.ptr(state), _lib.ptr(h), B, C, _strides(x, g, beta), float(decay_scale),
+                  _lib.ptr(state), _lib.ptr(h), B, C, _strides(x, g, beta), scale,
                   _lib.dtype_code(x.dtype), _lib.dtype_code(g.dtype), _lib.stream_of(x))
+    if not state.is_inference():  # a graph that kept the old state raises instead of using the new one
+        torch.autograd.graph.increment_version(state)
     return h
 
 

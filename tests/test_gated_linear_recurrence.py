@@ -179,6 +179,48 @@ def test_reset_starts_again(logits):
 
 
 @gpu
+def test_step_marks_its_state_as_changed():
+    """A graph that saved the state in front of a step raises instead of using the state behind it."""
+    x, state = torch.rand(2, 8, device=DEV), torch.rand(2, 8, device=DEV)
+    w = torch.rand(2, 8, device=DEV, requires_grad=True)
+    y = (w * state).sum()
+    with torch.no_grad():
+        gated_linear_recurrence_step(x, x, x, state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        state = torch.zeros(2, 8, device=DEV)
+        assert torch.equal(gated_linear_recurrence_step(x, x, x, state), state)
+
+
+@gpu
+@pytest.mark.parametrize("B,L", [(1, 700), (64, 300)])
+@pytest.mark.parametrize("logits", [False, True])
+def test_nothing_crosses_a_reset(logits, B, L):
+    """NaN and infinity on one side of a reset (few slabs: clusters; many: chains): the other side is as
+    it is without them, bit for bit, forward and backward."""
+    v = _inputs(B, L, 256, torch.float32, torch.float32, logits)
+    v["reset"] = torch.zeros(B, L, dtype=torch.bool)
+    v["reset"][:, 130] = v["reset"][:, 0] = True
+    clean = _run(v, 8.0)
+    w = {k: (t.clone() if t is not None else None) for k, t in v.items()}
+    w["x"][:, 100:130] = float("nan")
+    w["h0"][:] = float("inf")
+    got = _run(w, 8.0)
+    for k in ("h", "dx", "dg", "dbeta"):
+        assert torch.equal(got[k][:, 130:], clean[k][:, 130:]), k
+    assert torch.equal(got["h"][:, :100], clean["h"][:, :100])
+    assert torch.equal(got["hT"], clean["hT"])
+    w = {k: (t.clone() if t is not None else None) for k, t in v.items()}
+    w["dh"][:, 140:160] = float("nan")
+    w["dhT"][:] = float("inf")
+    got = _run(w, 8.0)
+    for k in ("h", "dx", "dg", "dbeta"):
+        assert torch.equal(got[k][:, :130], clean[k][:, :130]), k
+    assert bool((got["dh0"] == 0).all()) and bool((clean["dh0"] == 0).all())
+
+
+@gpu
 def test_reset_everywhere_and_nowhere():
     v = _inputs(2, 130, 40, torch.float32, torch.float32, True)
     v["reset"] = torch.ones(2, 130, dtype=torch.bool)
@@ -519,6 +561,14 @@ def test_step_refusals(host):
         gated_linear_recurrence_step(_z(2, 1, 4), x, x, x)
     with pytest.raises(RuntimeError, match="not differentiable"):
         gated_linear_recurrence_step(x.clone().requires_grad_(), x, x, _z(2, 4))
+
+
+@pytest.mark.parametrize("scale", [-1.0, float("nan"), float("inf")])
+def test_decay_scale_refusals(host, scale):
+    with pytest.raises(ValueError, match="decay_scale"):
+        gated_linear_recurrence(*[_z(2, 3, 4)] * 3, _z(4), decay_scale=scale)
+    with pytest.raises(ValueError, match="decay_scale"):
+        gated_linear_recurrence_step(*[_z(2, 4)] * 4, _z(4), decay_scale=scale)
 
 
 def test_cpu_tensors_are_refused():
