@@ -184,3 +184,32 @@ def test_captured_decode_step():
         tok.fill_(t + 3)
         assert torch.equal(step(), got[t])
     assert torch.equal(state, after)
+
+
+@pytest.mark.parametrize("B,L", [(1, 1000), (64, 150)])
+def test_two_calls_at_once(B, L):
+    """The operators on two streams, interleaved: each bit for bit as alone (no library product among
+    them; few rows take clusters, many take chains)."""
+    ids, _, reset = _batch(B, L)
+    ids, reset = ids.to(DEV), reset.to(DEV)
+    sets = [{n: t.to(DEV).mul(1 + k / 8).requires_grad_() for n, t in _params().items()} for k in (0, 1)]
+
+    def work(p):
+        r = scaled_embedding(ids, p["emb"], math.sqrt(N))
+        h = gated_linear_recurrence(r, r, r, p["decay"], decay_scale=SCALE, reset=reset)
+        out, res = residual_rms_norm(h, r, p["wa"], post_weight=p["posta"], gate=r, scale=p["sa"], eps=EPS)
+        used = [p[k] for k in ("emb", "decay", "wa", "posta", "sa")]
+        return [out.detach(), res.detach(), *torch.autograd.grad((out, res), used, (out.detach(), r.detach()))]
+    alone = [work(p) for p in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(4):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((k, work(sets[k])))
+    torch.cuda.synchronize()
+    for k, out in got:
+        for a, b in zip(out, alone[k]):
+            assert torch.equal(a, b)
