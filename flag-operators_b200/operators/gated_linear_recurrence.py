@@ -17,7 +17,8 @@ values near 1 need fp32: bf16 has no number between 0.996 and 1).  x, g and beta
 views whose last dimension is contiguous, such as column blocks of one projection; anything
 else is copied.  h has x's dtype; states are fp32 [B, C].
   initial_state   the state before the first token (zeros if None)
-  reset           bool [B, L]: steps that start again from nothing (a_t = 0), for packed sequences
+  reset           bool [B, L]: steps that start again from nothing (a_t = 0), for packed sequences;
+                  nothing in front of such a step reaches it, NaN and infinite gates included
   output_final_state   also return the state after the last token
 
 Gates above 1 make the state grow; their product over any 128 consecutive steps has to stay

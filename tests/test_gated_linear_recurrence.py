@@ -520,6 +520,46 @@ def test_double_backward_is_refused():
         dx.sum().backward()
 
 
+@gpu
+@pytest.mark.parametrize("B,L", [(1, 700), (64, 300)])
+@pytest.mark.parametrize("logits,bad", [(False, "nan"), (False, "inf"), (False, "growing"), (True, "nan")])
+def test_bad_gates_do_not_cross_a_reset(logits, bad, B, L):
+    """Gates that are NaN or infinite, or whose product leaves the fp32 range, among the steps that a
+    warp has with the reset: the other document is as it is without them."""
+    v = _inputs(B, L, 256, torch.float32, torch.float32, logits)
+    v["reset"] = torch.zeros(B, L, dtype=torch.bool)
+    v["reset"][:, 130] = True
+    value = {"nan": float("nan"), "inf": float("inf"), "growing": 1e25}[bad]
+
+    def with_gates(u, steps):
+        u = dict(u, g=u["g"].clone())
+        u["g"][:, steps] = value
+        return u
+    front = dict(v)
+    if bad == "growing":
+        front["x"], front["h0"] = v["x"].clone(), torch.zeros_like(v["h0"])
+        front["x"][:, :130] = 0
+        front["x"][:, 127] = 1e-30
+    clean = _run(front, 8.0)
+    for steps in ([128], [129], [128, 129], list(range(100, 130))):
+        got = _run(with_gates(front, steps), 8.0)
+        for k in ("h", "dx", "dg", "dbeta"):
+            assert torch.equal(got[k][:, 130:], clean[k][:, 130:]), (k, steps)
+        assert torch.equal(got["h"][:, :steps[0]], clean["h"][:, :steps[0]]), steps
+        assert torch.equal(got["hT"], clean["hT"]), steps
+    behind = dict(v)
+    if bad == "growing":
+        behind["dh"], behind["dhT"] = v["dh"].clone(), torch.zeros_like(v["dhT"])
+        behind["dh"][:, 130:] = 0
+        behind["dh"][:, 140] = 1e-30
+    clean = _run(behind, 8.0)
+    for steps in ([131], [133], [131, 132, 135], list(range(131, 160))):
+        got = _run(with_gates(behind, steps), 8.0)
+        for k in ("h", "dx", "dg", "dbeta"):
+            assert torch.equal(got[k][:, :130], clean[k][:, :130]), (k, steps)
+        assert torch.equal(got["dh0"], clean["dh0"]), steps
+
+
 # ---------------------------------------------------------------------------
 # refusals, on the CPU: nothing reaches the library
 # ---------------------------------------------------------------------------
