@@ -715,8 +715,8 @@ glr_bwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
             const F mi = ring.mi[w][i][lane], ci = ring.get_gates(s, w, i, lane);
             b = mul_(mi, xv);
             F du = mul_(D[i], fma_(a[i], hv, mul_(mul_(ring.q[w][i][lane], b), all_<F>(-1.f))));
-            if (zero) du = all_<F>(0.f);
             du = mul_(du, u[i]);
+            if (zero) du = all_<F>(0.f);  // whatever u is
             if (full || i < n) sum = add_(sum, du);
             og = mul_(du, c[i]);
             ox = mul_(D[i], mi);

@@ -560,6 +560,24 @@ def test_bad_gates_do_not_cross_a_reset(logits, bad, B, L):
         assert torch.equal(got["dh0"], clean["dh0"]), steps
 
 
+@gpu
+@pytest.mark.parametrize("B", [1, 64])
+@pytest.mark.parametrize("logits", [False, True])
+def test_the_gate_of_a_reset_step_is_not_used(logits, B):
+    """a_t is 0 there whatever g_t is, NaN and infinity included, and g_t's gradient is 0."""
+    v = _inputs(B, 300, 256, torch.float32, torch.float32, logits)
+    v["reset"] = torch.zeros(B, 300, dtype=torch.bool)
+    v["reset"][:, 0] = v["reset"][:, 130] = v["reset"][:, 131] = True
+    clean = _run(v, 8.0)
+    for value in (float("nan"), float("inf"), float("-inf")):
+        w = dict(v, g=v["g"].clone())
+        w["g"][:, 0] = w["g"][:, 130] = w["g"][:, 131] = value
+        got = _run(w, 8.0)
+        assert bool((got["dg"][v["reset"]] == 0).all()), value
+        for k in got:
+            assert torch.equal(got[k], clean[k]), (k, value)
+
+
 # ---------------------------------------------------------------------------
 # refusals, on the CPU: nothing reaches the library
 # ---------------------------------------------------------------------------
