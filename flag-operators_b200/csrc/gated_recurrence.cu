@@ -87,13 +87,6 @@ __device__ __forceinline__ float rsqrt_(float x) {
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// min that keeps a NaN
-__device__ __forceinline__ float min_nan(float x, float y) {
-  float z;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
-  return z;
-}
-
 // softplus(decay), the rate of a fully open gate
 __device__ __forceinline__ float softplus(float decay) {
   return decay > 20.f ? decay : log1pf(expf(decay));
@@ -446,18 +439,19 @@ glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
       const F gv = EG::load(&ring.g[s][w][(i * 32 + lane) * EG::kBytes]);
       const F bv = EG::load(&ring.b[s][w][(i * 32 + lane) * EG::kBytes]);
       if (LOGITS) {
-        // sigmoid(g) = 1 / (1 + e^-g), 0 and 1 at -inf and +inf; m i = sqrt(v) / q with v = 1 - a^2 and
-        // q = 1 + e^-beta (kept below 2^60) is v rsqrt(v q^2), which saves one of six of the slow
-        // instructions (exponentials, reciprocals, roots) that bound this kernel.
+        // sigmoid(g) = 1 / (1 + e^-g), 0 and 1 at -inf and +inf.  With v = 1 - a^2, r = e^-|beta| and
+        // q = 1 + r, m i is sqrt(v) / q, times r where beta is negative; sqrt(v) / q = v rsqrt(v q^2) saves
+        // one of six of the slow instructions (exponentials, reciprocals, roots) that bound this kernel.
         const F sg = map_(rcp, add_(map_(ex2, mul_(gv, all_<F>(-kLog2e))), all_<F>(1.f)));
         a[i] = map_(ex2, mul_(sg, r1));
         F v = one_minus_exp(mul_(sg, r2), mul_(a[i], a[i]));
         if (RESET && (rs >> i & 1)) v = all_<F>(1.f);
-        const F q = add_(map_([](float t) { return ex2(min_nan(t, 60.f)); }, mul_(bv, all_<F>(-kLog2e))),
-                         all_<F>(1.f));
+        const F e = mul_(bv, all_<F>(kLog2e));
+        const F r = map_([](float t) { return ex2(-fabsf(t)); }, e), q = add_(r, all_<F>(1.f));
+        const F xr = mul_(xv, map_([](float t, float r_) { return t < 0.f ? r_ : 1.f; }, e, r));
         // 1e-36: no root of 0 where a == 1, and v then makes the product 0
         const F t = map_(rsqrt_, fma_(mul_(v, q), q, all_<F>(1e-36f)));
-        b[i] = mul_(mul_(v, t), xv);
+        b[i] = mul_(mul_(v, t), xr);
       } else {
         a[i] = gv;
         b[i] = mul_(bv, xv);

@@ -578,6 +578,42 @@ def test_the_gate_of_a_reset_step_is_not_used(logits, B):
             assert torch.equal(got[k], clean[k]), (k, value)
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_closed_input_gates(dtype):
+    """Input gates far closed, over an empty state, where h is b = m i x alone.  beta log2(e) is rounded
+    twice, which is 2 |beta| U of its exponential, and the rest of b carries 16 U; forward and step are
+    each within that of the formula.  What is below the smallest normal number may be 0, and -inf is 0."""
+    beta = torch.tensor([-30., -41.5, -41.7, -44.5, -50., -64., -80., -87.2, -200., float("-inf")])
+    B = len(beta)
+    v = _inputs(B, 40, 64, dtype, dtype, True)
+    v["beta"] = beta[:, None, None].expand(B, 40, 64).to(dtype).contiguous()
+    v["h0"].zero_()
+    i = torch.sigmoid(v["beta"].double())
+    size = torch.where(torch.isinf(v["beta"]), torch.zeros(()), v["beta"].float()).abs().double()
+    on = {k: t.to(DEV) for k, t in v.items() if t is not None}
+    want = i * v["x"].double()  # m is 1 where every step starts again
+    got = gated_linear_recurrence(on["x"], on["g"], on["beta"], on["decay"], decay_scale=8.0,
+                                  reset=torch.ones(B, 40, dtype=torch.bool, device=DEV))
+    _within(got, want, (2 * size + 16) * U * want.abs(), "h, every step a reset")
+    assert bool((got[-1] == 0).all())
+    u = -8 * torch.nn.functional.softplus(v["decay"].double()) * torch.sigmoid(v["g"].double())
+    want = (torch.sqrt(-torch.expm1(2 * u)) * want)[:, 0]
+    tol = (2 * size[:, 0] + 16) * U * want.abs()
+    got = gated_linear_recurrence(on["x"][:, :1], on["g"][:, :1], on["beta"][:, :1], on["decay"],
+                                  decay_scale=8.0)[:, 0]
+    _within(got, want, tol, "h, one step")
+    state = torch.zeros(B, 64, device=DEV)
+    step = gated_linear_recurrence_step(on["x"][:, 0], on["g"][:, 0], on["beta"][:, 0], state, on["decay"],
+                                        decay_scale=8.0)
+    _within(step, want, tol, "step")
+    assert bool((got[-1] == 0).all()) and bool((step[-1] == 0).all())
+    # a NaN is no closed gate
+    on["beta"][:, 7] = float("nan")
+    got = gated_linear_recurrence(on["x"], on["g"], on["beta"], on["decay"], decay_scale=8.0)
+    assert bool(torch.isnan(got[:, 7:]).all()) and bool(torch.isfinite(got[:, :7]).all())
+
+
 # ---------------------------------------------------------------------------
 # refusals, on the CPU: nothing reaches the library
 # ---------------------------------------------------------------------------
