@@ -254,6 +254,9 @@ __device__ __forceinline__ float inv_sqrt(float x) {
   return x < INFINITY ? r * fmaf(-0.5f * x * r, r, 1.5f) : r;
 }
 
+// inv^3 x, for an x of about 1 / inv: inv^3 alone leaves the fp32 range for rows of norm 1e13 and 1e-13.
+__device__ __forceinline__ float cubed(float inv, float x) { return inv * (inv * (inv * x)); }
+
 // Bytes of two fp32 weight vectors of N elements, each a multiple of 16.
 __host__ __device__ constexpr int weight_bytes(int64_t N) { return (int)((N + 3) / 4 * 4 * 8); }
 
@@ -489,8 +492,8 @@ rrn_bwd_kernel(Bwd a) {
     }
     float sum[3] = {s1.x + s1.y, s2.x + s2.y, s3.x + s3.y};
     row_sum<TPR, CTAS>(sum, red + 3 * s);
-    const float c2 = inv2 * inv2 * inv2 * (sum[0] * rn);
-    const float c1 = a.wp ? inv1 * inv1 * inv1 * (fmaf(-c2, sum[2], sum[1]) * rn) : 0.f;
+    const float c2 = cubed(inv2, sum[0] * rn);
+    const float c1 = a.wp ? cubed(inv1, fmaf(-c2, sum[2], sum[1]) * rn) : 0.f;
     const float2 m2 = all_<float2>(-c2), m1 = all_<float2>(-c1);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -624,12 +627,12 @@ __global__ void __launch_bounds__(256) rrn_bwd_generic_kernel(Bwd a) {
       }
     }
     s1 = block_sum(s1, red);
-    const float c2 = inv2 * inv2 * inv2 * s1 / (float)a.N;
+    const float c2 = cubed(inv2, s1 / (float)a.N);
     float c1 = 0.f;
     if (wp) {
       s2 = block_sum(s2, red);
       s3 = block_sum(s3, red);
-      c1 = inv1 * inv1 * inv1 * fmaf(-c2, s3, s2) / (float)a.N;
+      c1 = cubed(inv1, fmaf(-c2, s3, s2) / (float)a.N);
     }
     if (threadIdx.x == 0) a.c2[row] = c2;
     for (int64_t j = threadIdx.x; j < a.N; j += blockDim.x) {

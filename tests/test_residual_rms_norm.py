@@ -317,6 +317,24 @@ def test_captured_replay_and_other_stream():
     assert all(torch.equal(o, want[k]) for k, o in zip(names, out))
 
 
+@gpu
+@pytest.mark.parametrize("N,dtype", [(256, torch.float32), (257, torch.float32), (8200, torch.float32),
+                                     (512, torch.bfloat16), (16384, torch.bfloat16)])
+@pytest.mark.parametrize("which", ["y", "residual"])
+def test_gradients_of_large_and_small_rows(N, dtype, which, monkeypatch):
+    """Rows whose norm's cube, or its reciprocal's, is outside the fp32 range.  Small ones want eps = 0:
+    the formulas' gradients then grow as the rows shrink."""
+    for size in (1e15, 1e-14):
+        monkeypatch.setitem(globals(), "EPS", 1e-6 if size > 1 else 0.0)
+        post = which == "y"
+        v, (do, dr) = _inputs(6, N, dtype, post=post)
+        v["y"][2] *= size
+        if not post:
+            v["residual"][2] *= size
+        for cot in ((do, dr), (do, None)):
+            _check(v, "silu", cot)
+
+
 # ---------------------------------------------------------------------------
 # on the CPU: the row view, refusals
 # ---------------------------------------------------------------------------
