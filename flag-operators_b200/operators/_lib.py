@@ -13,6 +13,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get(
@@ -177,6 +178,14 @@ def on_device(t: torch.Tensor):
     if t.get_device() == torch.cuda.current_device():
         return _SAME_DEVICE
     return torch.cuda.device(t.device)
+
+
+def refuse_tangents(op: str, *tensors: torch.Tensor | None) -> None:
+    """Raises where a tensor carries a forward-mode tangent, which a launch would lose."""
+    if forward_ad._current_level < 0:  # not under a dual level: a number to look at
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{op}: has no forward-mode derivative; use reverse mode")
 
 
 def i64_array(vals) -> ctypes.Array:

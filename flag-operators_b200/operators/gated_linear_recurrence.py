@@ -26,7 +26,7 @@ within the fp32 range (over an empty state it may leave it).
 A padded step that keeps the state (g = 1, beta = 0 as values; g = -inf as logits) must hold
 a finite x.  The state is fp32 throughout and h is rounded once.
 
-All of x, g, beta, decay and initial_state are differentiable, once (csrc/gated_recurrence.cu;
+All of x, g, beta, decay and initial_state are differentiable, once, in reverse mode (csrc/gated_recurrence.cu;
 the backward reads x, g, beta and dh and recomputes the states from fp32 checkpoints every
 64 steps).  gated_linear_recurrence_step is for decoding: x, g, beta [B, C], `state` [B, C] fp32
 is overwritten (it must not share memory with the other arguments), and nothing is differentiated.
@@ -155,6 +155,7 @@ def gated_linear_recurrence(
     logger.debug("FLAG-OPS GATED_LINEAR_RECURRENCE")
     op = "gated_linear_recurrence"
     _lib.require_cuda(x, op)
+    _lib.refuse_tangents(op, x, g, beta, decay, initial_state)
     if x.dim() != 3:
         raise ValueError(f"{op}: x must be [B, L, C], got shape {tuple(x.shape)}")
     scale = float(decay_scale)
@@ -196,6 +197,7 @@ def gated_linear_recurrence_step(
     """One token of every sequence: overwrites `state` with h_t and returns it in x's dtype."""
     op = "gated_linear_recurrence_step"
     _lib.require_cuda(x, op)
+    _lib.refuse_tangents(op, x, g, beta, decay, state)
     if x.dim() != 2:
         raise ValueError(f"{op}: x must be [B, C], got shape {tuple(x.shape)}")
     scale = float(decay_scale)

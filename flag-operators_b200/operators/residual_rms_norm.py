@@ -15,7 +15,7 @@ input and new_residual the stream to add its output to.  The second norm takes t
 before it is rounded to new_residual.  Row-strided views (column blocks of a projection) are read
 in place.
 
-Differentiable, once, in every tensor argument (csrc/residual_norm.cu); sums over rows are in
+Differentiable, once and in reverse mode, in every tensor argument (csrc/residual_norm.cu); sums over rows are in
 a fixed order.  A gate shared by several rows may be passed expanded: autograd adds its gradient up.
 """
 from __future__ import annotations
@@ -136,6 +136,8 @@ def residual_rms_norm(
     logger.debug("FLAG-OPS RESIDUAL_RMS_NORM")
     op = "residual_rms_norm"
     _lib.require_cuda(y, op)
+    _lib.refuse_tangents(op, y, residual, weight, post_weight, gate,
+                         scale if isinstance(scale, torch.Tensor) else None)
     if y.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise TypeError(f"{op}: dtype {y.dtype} is not supported")
     if y.dim() < 1 or y.shape[-1] < 1:

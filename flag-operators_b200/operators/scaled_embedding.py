@@ -13,7 +13,7 @@ other and get no gradient.
 
 As scatter_reduce does with its index, ids outside [0, V) are not read: they give a row of
 zeros and no gradient, and with FLAGOPS_CHECK_INDEX=1 the wrapper synchronises and raises
-IndexError.  scaled_embedding is differentiable, once, in weight.
+IndexError.  scaled_embedding is differentiable, once and in reverse mode, in weight.
 """
 from __future__ import annotations
 
@@ -102,6 +102,7 @@ def scaled_embedding(
     logger.debug("FLAG-OPS SCALED_EMBEDDING")
     op = "scaled_embedding"
     _lib.require_cuda(weight, op)
+    _lib.refuse_tangents(op, weight)
     if weight.dim() != 2:
         raise ValueError(f"{op}: weight must be [V, N], got shape {tuple(weight.shape)}")
     _check_dtype(op, weight)
@@ -129,6 +130,7 @@ def scaled_embedding_backward(
     """d weight [num_embeddings, N] of scaled_embedding, in dout's dtype."""
     op = "scaled_embedding_backward"
     _lib.require_cuda(dout, op)
+    _lib.refuse_tangents(op, dout)
     _check_dtype(op, dout)
     V = int(num_embeddings)
     if V < 0 or dout.dim() < 1 or dout.shape[:-1] != ids.shape:

@@ -665,6 +665,22 @@ def test_decay_scale_refusals(host, scale):
         gated_linear_recurrence_step(*[_z(2, 4)] * 4, _z(4), decay_scale=scale)
 
 
+def test_tangents_are_refused(host):
+    """A dual tensor would lose its tangent in a launch."""
+    fw = torch.autograd.forward_ad
+    with fw.dual_level():
+        for k in range(5):
+            a = [_z(2, 3, 4), _z(2, 3, 4), _z(2, 3, 4), _z(4), _z(2, 4)]
+            a[k] = fw.make_dual(a[k], torch.ones_like(a[k]))
+            with pytest.raises(RuntimeError, match="gated_linear_recurrence: has no forward-mode"):
+                gated_linear_recurrence(*a[:4], initial_state=a[4])
+            a = [_z(2, 4), _z(2, 4), _z(2, 4), _z(2, 4), _z(4)]
+            a[k] = fw.make_dual(a[k], torch.ones_like(a[k]))
+            with pytest.raises(RuntimeError, match="_step: has no forward-mode"):
+                gated_linear_recurrence_step(*a)
+        _lib.refuse_tangents("op", _z(2, 4), None)  # under a level, without a tangent
+
+
 def test_cpu_tensors_are_refused():
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         gated_linear_recurrence(*[_z(1, 2, 4)] * 3)

@@ -385,6 +385,17 @@ def test_refusals(host, err, args, kw):
         residual_rms_norm(*args, **kw)
 
 
+def test_tangents_are_refused(host):
+    """A dual tensor would lose its tangent in a launch."""
+    fw = torch.autograd.forward_ad
+    with fw.dual_level():
+        for k in range(6):
+            a = [_z(2, 4), _z(2, 4), _z(4), _z(4), _z(2, 4), _z(4)]
+            a[k] = fw.make_dual(a[k], torch.ones_like(a[k]))
+            with pytest.raises(RuntimeError, match="residual_rms_norm: has no forward-mode"):
+                residual_rms_norm(*a[:3], post_weight=a[3], gate=a[4], scale=a[5])
+
+
 def test_cpu_tensors_are_refused():
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         residual_rms_norm(_z(2, 4), _z(2, 4), _z(4))

@@ -266,6 +266,17 @@ def test_checked_ids_raise_before_the_library(host, monkeypatch):
         scaled_embedding_backward(torch.zeros(1, 2), torch.tensor([-1]), 4)
 
 
+def test_tangents_are_refused(host):
+    """A dual tensor would lose its tangent in a launch."""
+    fw = torch.autograd.forward_ad
+    i, w, d = torch.zeros(3, dtype=torch.int64), torch.zeros(4, 2), torch.zeros(3, 2)
+    with fw.dual_level():
+        with pytest.raises(RuntimeError, match="scaled_embedding: has no forward-mode"):
+            scaled_embedding(i, fw.make_dual(w, torch.ones_like(w)))
+        with pytest.raises(RuntimeError, match="scaled_embedding_backward: has no forward-mode"):
+            scaled_embedding_backward(fw.make_dual(d, torch.ones_like(d)), i, 4)
+
+
 def test_cpu_tensors_are_refused():
     i, w = torch.zeros(3, dtype=torch.int64), torch.zeros(4, 2)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
