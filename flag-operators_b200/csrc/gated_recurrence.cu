@@ -87,9 +87,14 @@ __device__ __forceinline__ float rsqrt_(float x) {
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// softplus(decay), the rate of a fully open gate
 __device__ __forceinline__ float softplus(float decay) {
   return decay > 20.f ? decay : log1pf(expf(decay));
+}
+// -log a of a fully open gate.  Kept finite: times a closed gate's 0, and the gradient's 0 where a is 0,
+// it has to be 0.
+__device__ __forceinline__ float rate_of(float scale, float decay) {
+  const float r = scale * softplus(decay);
+  return r > 1e30f ? 1e30f : r;
 }
 
 // The state s behind a segment that maps it to A s + H.  Where a segment may hold a reset (A is 0),
@@ -405,7 +410,7 @@ glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
   F S = all_<F>(0.f);
   if (p.on) {
     if (LOGITS) {
-      const F rate = map_([&](float d) { return scale * softplus(d); },
+      const F rate = map_([&](float d) { return rate_of(scale, d); },
                           Elem<float, V>::load(decay + p.c));
       r1 = mul_(rate, all_<F>(-kLog2e));
       r2 = mul_(rate, all_<F>(2.f));
@@ -582,7 +587,7 @@ glr_bwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
   F R = all_<F>(0.f);  // a_t D_t of the step behind the round
   if (p.on) {
     if (LOGITS)
-      rate = map_([&](float d) { return -scale * softplus(d); }, Elem<float, V>::load(decay + p.c));
+      rate = map_([&](float d) { return -rate_of(scale, d); }, Elem<float, V>::load(decay + p.c));
     if (dhT) R = Elem<float, V>::load(dhT + p.b * C + p.c);
   }
   auto rows_of = [&](int64_t t) { return t >= 0 && t < L ? (int)(L - t < N ? L - t : N) : 0; };
@@ -779,7 +784,7 @@ glr_step_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __res
                 int64_t B, int64_t C, Strides st, float scale) {
   const int64_t c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (c >= C) return;
-  const float rate = LOGITS ? -scale * softplus(decay[c]) : 0.f;
+  const float rate = LOGITS ? -rate_of(scale, decay[c]) : 0.f;
   for (int64_t b = blockIdx.y; b < B; b += gridDim.y) {
     float a = to_f<G>(g[b * st.gb + c]), in = to_f<G>(beta[b * st.bb + c]);
     if (LOGITS) {

@@ -614,6 +614,31 @@ def test_closed_input_gates(dtype):
     assert bool(torch.isnan(got[:, 7:]).all()) and bool(torch.isfinite(got[:, :7]).all())
 
 
+@gpu
+def test_rates_beyond_the_fp32_range():
+    """decay or decay_scale times its softplus infinite in fp32: an open gate forgets all (a = 0, m = 1), a
+    closed one nothing (a = 1, m = 0), and neither has a slope."""
+    v = _inputs(2, 150, 64, torch.float32, torch.float32, True)
+    v["g"][:, ::3] = float("-inf")
+    i = torch.sigmoid(v["beta"].double())
+    want, now = [], v["h0"].double()
+    for t in range(150):
+        now = now if t % 3 == 0 else i[:, t] * v["x"][:, t].double()
+        want.append(now)
+    want = torch.stack(want, 1)
+    for scale, decay in ((8.0, float("inf")), (3e38, 5.0)):
+        v["decay"].fill_(decay)
+        got = _run(v, scale)
+        _within(got["h"], want, 20 * U * want.abs(), "h")
+        assert all(bool(torch.isfinite(t).all()) for t in got.values())
+        assert bool((got["dg"] == 0).all()) and bool((got["ddecay"] == 0).all())
+        state = v["h0"].to(DEV)
+        for t in range(2):
+            o = gated_linear_recurrence_step(*(v[k][:, t].to(DEV) for k in ("x", "g", "beta")), state,
+                                             v["decay"].to(DEV), decay_scale=scale)
+            _within(o, want[:, t], 20 * U * want[:, t].abs(), "step")
+
+
 # ---------------------------------------------------------------------------
 # refusals, on the CPU: nothing reaches the library
 # ---------------------------------------------------------------------------
