@@ -10,7 +10,8 @@
 //     a chunk by id in shared memory (stable, 9 bits of the id a pass).  Ids that do not count
 //     get the key V.  No chunk waits for another.
 //  2. emb_merge_kernel (more than one chunk): a token's place in the order of all chunks is its
-//     place in its own plus the numbers of smaller keys in the others, found by bisection.
+//     place in its own plus the numbers of smaller keys in the others, found by bisection: T^2 / kChunk
+//     bisections, where all else is linear in T.
 //  3. emb_piece_kernel: a CTA adds up 32 consecutive sorted tokens, whatever their ids: each row of
 //     dout is read once, and an id with many tokens (padding, frequent words) costs no CTA more
 //     than 32.  Rows of dW whose tokens all lie in the piece are written, the sums of the ids
@@ -25,7 +26,9 @@
 // pieces, 4 us runs, 11 us join, which is 1.25 GB at 5.6 TB/s.  Finding each row's tokens in the
 // kernel that writes dW was slower (241 us for that kernel alone: its CTAs wait for bounds,
 // positions and rows one after the other).  30011 tokens, a third of them one id, 5003 x 771 fp32:
-// 27 us and 74 us; there the bisections and the unaligned rows' 4-byte accesses count.
+// 27 us and 74 us; there the bisections and the unaligned rows' 4-byte accesses count.  Gradients of
+// 32000 x 1024 bf16: 53 us with 16384 tokens, 97 with 65536, 162 with 131072, 326 with 262144, of
+// which the merge is more than half, and 2.4 ms with 1048576, of which it is 1.9.
 #include <type_traits>
 
 #include "common.cuh"

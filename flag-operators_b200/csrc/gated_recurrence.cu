@@ -24,8 +24,8 @@
 // and it walks them once, from the state that enters them.  That state comes
 //  - where slabs * B give every SM a CTA: from the neighbouring warp, as a chain through shared memory
 //    (an mbarrier a link), so that warps run ahead of one another and the gates of one overlap the
-//    walk of another: 235 us against 266 us with a barrier for all warps, forward at 8 x 8192 x 2048
-//    bf16 logits;
+//    walk of another (235 us against 266 us with a barrier for all warps when it came, forward at
+//    8 x 8192 x 2048 bf16 logits; 242 us now);
 //  - with fewer slabs: up to 8 CTAs of a cluster take consecutive tiles, each warp's map is put
 //    together with those in front of it, and the CTAs exchange theirs as asynchronous stores that an
 //    mbarrier of the receiver counts (a cluster barrier waits for the outputs' stores too: backward
@@ -33,11 +33,12 @@
 // Inputs come through a ring of two rounds in shared memory (cp.async), which each warp fills and reads
 // by itself.  Every input is read once and every output written once.
 //
-// What bounds it (1 x B200, bf16): gates as values run at the memory's rate (forward 160 us at
-// 8 x 8192 x 2048, 1.07 GB).  With logits an element takes five exponentials, reciprocals and roots,
-// which alone take 150 us there: 235 us forward (floor 164).  Backward 500 us (floor 287): 140
-// instructions for a pair of channels at 55 % of the issue rate, 16 warps on an SM (its shared
-// memory is full).  Both lose an eighth to 256 CTAs on 148 SMs.
+// What bounds it (1 x B200, 8 x 8192 x 2048 bf16): gates as values 198 us forward and 355 us backward
+// (floors 164 and 287 us at the measured rate of a copy), with fp32 gates 268 and 570 (246 and 451).
+// With logits an element takes five exponentials, reciprocals and roots, which alone take 150 us:
+// 242 us forward, 505 us backward (140 instructions for a pair of channels at 55 % of the issue rate, and
+// no more than 16 warps on an SM: two CTAs of 256 threads with up to 128 registers are all its
+// registers).  fp32 logits 316 and 730 us.  All of them lose an eighth to 256 CTAs on 148 SMs.
 
 #include <type_traits>
 
@@ -47,9 +48,9 @@
 namespace fo {
 namespace {
 
-// Steps of a thread in a round, and warps of a CTA.  Forward at 8 x 8192 x 2048 bf16: 235 us; with
-// 8 steps and 16 warps 239, 8 and 8 267, 16 and 12 263, 4 and 16 288.  Backward needs the registers
-// for 8 steps.
+// Steps of a thread in a round, and warps of a CTA.  Forward at 8 x 8192 x 2048 bf16, in one comparison:
+// 235 us; with 8 steps and 16 warps 239, 8 and 8 267, 16 and 12 263, 4 and 16 288.  Backward needs the
+// registers for 8 steps.
 constexpr int kFwdSteps = 16, kFwdWarps = 8;
 constexpr int kFwdTile = kFwdSteps * kFwdWarps;
 constexpr int kBwdSteps = 8, kBwdWarps = 8;
@@ -522,7 +523,8 @@ template <typename T, typename G, int V> struct BwdRing {
   uint8_t g[kStages][kBwdWarps][Stream<G, V, kBwdSteps>::kBytes];
   uint8_t b[kStages][kBwdWarps][Stream<G, V, kBwdSteps>::kBytes];
   // Of the round between its first and last walk, where registers would spill: m i and
-  // a^2 / (1 - a^2); 1 - i takes the place of g and beta in the ring.
+  // a^2 / (1 - a^2); 1 - i takes the place of g and beta in the ring.  Gates as values do not need
+  // them; leaving them out would admit no further CTA, since registers limit the number first.
   F mi[kBwdWarps][kBwdSteps][32], q[kBwdWarps][kBwdSteps][32];
 
   // one F a lane in the places of g and beta of step i, which are not needed any more
@@ -931,8 +933,8 @@ extern "C" int fo_glr_fwd(const void* x, const void* g, const void* beta, const 
     const bool two = pairs_ok(xs, 2, gs, 2, fs, 4, q, C, sizeof(T), sizeof(G));
     const bool wide = wide_ok(xs, 1, gs, 2, q, C, sizeof(T), sizeof(G));
     const int64_t ctas = B * slabs_of(C, two ? 2 : 1);
-    // CTAs of a cluster until every SM has one: 266 us without, 294 with two at 8 x 8192 x 2048 bf16,
-    // where there are 256 CTAs as it is.
+    // CTAs of a cluster until every SM has one: 242 us without, 292 with two at 8 x 8192 x 2048 bf16, where
+    // there are 256 CTAs as it is; 242 and 228 with 160 or 192 CTAs (batches of 5 and 6).
     const int cl = cluster_for(ctas, (L + kFwdTile - 1) / kFwdTile, num_sms(), kMostCtas);
     return with_flags(two, decay, reset, [&](auto tw, auto lo, auto rs) {
       constexpr int V = tw && sizeof(G) == 2 ? 2 : 1;

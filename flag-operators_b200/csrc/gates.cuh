@@ -96,7 +96,9 @@ __device__ __forceinline__ float2 map_(Fn f, float2 a, float2 b, float2 c) {
 }
 
 // sigmoid(z) and 1 - sigmoid(z), neither with cancellation: e = e^-z, s = 1 / (1 + e), c = e s, which
-// is 1 (fmin passes over the NaN of inf * 0) where e is infinite.
+// is 1 (fmin passes over the NaN of inf * 0) where e is infinite.  For e of 2^126 and more (z below
+// -87.3) the reciprocal flushes s to 0, and c is 0 with it until e is infinite (z below -88.7): only
+// for callers that take c times s, or times what has s as a factor, as all here do.
 template <typename F> __device__ __forceinline__ void sigmoid_pair(F z, F& s, F& c) {
   const F e = map_(ex2, mul_(z, all_<F>(-kLog2e)));
   s = map_(rcp, add_(e, all_<F>(1.f)));

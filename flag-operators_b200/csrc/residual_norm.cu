@@ -26,10 +26,12 @@
 // and w are kept in shared memory in fp32.
 //
 // Measured (B200): 16384 x 8192 bf16 with gate and both norms 237 us forward (5 streams, 1.34 GB,
-// 5.7 TB/s) and 430 us backward (8 streams, 5.0 TB/s; 59 instructions an element at half the issue
-// rate, one CTA of 512 threads on an SM); 4096 x 4096 fp32 48 and 62 us; 4096 x 16384 bf16 150 and
-// 265 us.  1024 threads with one vector each were slower (297 us forward), and so was the backward
-// with 64 registers (740 us: it spills).
+// 5.7 TB/s) and 423 us backward (8 streams, 5.1 TB/s; 59 instructions an element at half the issue
+// rate, one CTA of 512 threads on an SM) and 6 for the column sums; 4096 x 4096 fp32 without a gate 49,
+// 63 and 5 us; 4096 x 16384 bf16 150 and 270 us.  1024 threads with one vector each were slower (297 us
+// forward), and so was the backward with 64 registers (740 us: it spills).  The generic kernels are far
+// from the memory's rate: 4096 x 12288 fp32 877 us forward, 799 + 191 backward (154 and 246 at a copy's
+// rate), 4096 x 5001 bf16 241 us and 281 + 81 (31 and 50).
 
 #include <type_traits>
 

@@ -226,7 +226,8 @@ def gated_linear_recurrence_step(
 
 
 def timeouts() -> int:
-    """Waits between CTAs that ran out of polls since the library was loaded (0 in a healthy run)."""
+    """Threads that gave up a wait between CTAs or warps on the current device since the library was
+    loaded (0 in a healthy run; the outputs of such a call are not complete)."""
     c = ctypes.c_uint(0)
     _lib.call("fo_glr_timeouts", ctypes.byref(c))
     return int(c.value)

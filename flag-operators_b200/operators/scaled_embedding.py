@@ -7,7 +7,8 @@
 
 ids: int64 or int32 of any shape; weight: [V, N] fp32 / fp16 / bf16.  The product is taken in
 fp32 and rounded once; the gradient's sums are in fp32 and in a fixed order (tokens sorted by id,
-no floating-point atomics), so it is the same in every run.  The gradient is dense: all of its
+no floating-point atomics), so it is the same in every run.  Its time grows with the square of the
+tokens from some 100000 on (2.4 ms for 2^20 of 1024 channels).  The gradient is dense: all of its
 V rows are written.  Rows of `padding_idx` (negative counts from the end) are looked up as any
 other and get no gradient.
 

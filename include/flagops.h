@@ -425,9 +425,9 @@ FO_API int fo_glr_bwd(const void* x, const void* g, const void* beta, const floa
                       int64_t L, int64_t C, const int64_t* strides, float scale, int dtype,
                       int gate_dtype, void* workspace, int64_t ws_bytes, void* stream);
 
-/* Number of waits between the CTAs of a cluster that ran out of polls since the library was loaded
- * (0 in a healthy run; such a call's outputs are not complete).  Synchronous read of a device
- * counter. */
+/* Waits that ran out of polls since the library was loaded, between the CTAs of a cluster or the warps
+ * of a CTA, counted by every thread that gave up (0 in a healthy run; such a call's outputs are not
+ * complete).  Synchronous read of a counter of the current device. */
 FO_API int fo_glr_timeouts(unsigned int* count);
 
 /* ------------------------------------------------------------------------ */
@@ -474,7 +474,8 @@ FO_API int fo_embedding_fwd(const void* ids, const void* weight, void* out, int6
 /*
  * dw[v, :] = scale * sum of dout[t, :] over the t with ids[t] == v, in fp32 and in a fixed order;
  * every row of dw [V, N] is written.  Ids outside [0, V) and equal to padding_idx add nothing
- * (padding_idx -1: none).
+ * (padding_idx -1: none).  Time grows with T^2 from some 100000 tokens on (2.4 ms for 2^20 of
+ * 1024 channels).
  */
 FO_API int fo_embedding_bwd_workspace_bytes(int64_t T, int64_t V, int64_t N, int64_t* bytes);
 FO_API int fo_embedding_bwd(const void* dout, const void* ids, void* dw, int64_t T, int64_t V,
