@@ -65,17 +65,25 @@ struct Strides {
   int64_t xb, xl, gb, gl, bb, bl;  // batch and step strides of x, g, beta, in elements
 };
 
-// (1 - e^{-w}) / w on [0, 1/2]: interpolation at the six Chebyshev nodes, relative error 3e-9.
-// Above 1/2 the subtraction 1 - e^{-w} loses at most a factor 2.5; below, it would lose 1 / w.
-template <typename F>
-__device__ __forceinline__ F one_minus_exp(F w, F e) {
+// a b, rounded: the compiler does not make it part of an fma, so that single values and pairs agree
+__device__ __forceinline__ float product(float a, float b) { return __fmul_rn(a, b); }
+__device__ __forceinline__ float2 product(float2 a, float2 b) { return mul_(a, b); }
+
+// v = 1 - e^{-w} for w = 2 y, from a near e^{-y} on the way in.  Up to w = 1/2 it is w p(w), p the
+// interpolation of (1 - e^{-w}) / w at the six Chebyshev nodes, relative error 3e-9: 1 - a^2 would lose 1 / w
+// there, above it loses at most a factor 2.5.  And a, an approximate exponential, is up to 2 units of its
+// last place off, mostly to one side, which a state that remembers 1 / (1 - a) steps would gather: it is
+// mended by half of what 1 - a^2 (rounded once) differs from v (1 / (2 a) of it for a near 1).
+template <typename F> __device__ __forceinline__ F one_minus_square(F w, F& a) {
   F p = fma_(w, all_<F>(-1.1234042e-3f), all_<F>(8.1896139e-3f));
   p = fma_(w, p, all_<F>(-4.1630074e-2f));
   p = fma_(w, p, all_<F>(0.16666242f));
   p = fma_(w, p, all_<F>(-0.49999982f));
   p = fma_(w, p, all_<F>(1.f));
-  return map_([](float w_, float s, float l) { return w_ < 0.5f ? s : l; }, w, mul_(w, p),
-              fma_(e, all_<F>(-1.f), all_<F>(1.f)));
+  const F f = fma_(a, a, all_<F>(-1.f));  // a^2 - 1
+  const F v = map_([](float w_, float s, float l) { return w_ < 0.5f ? s : -l; }, w, product(w, p), f);
+  a = fma_(add_(f, v), all_<F>(-0.5f), a);
+  return v;
 }
 __device__ __forceinline__ float sqrt_(float x) {
   float y;
@@ -450,7 +458,7 @@ glr_fwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
         // one of six of the slow instructions (exponentials, reciprocals, roots) that bound this kernel.
         const F sg = map_(rcp, add_(map_(ex2, mul_(gv, all_<F>(-kLog2e))), all_<F>(1.f)));
         a[i] = map_(ex2, mul_(sg, r1));
-        F v = one_minus_exp(mul_(sg, r2), mul_(a[i], a[i]));
+        F v = one_minus_square(mul_(sg, r2), a[i]);
         if (RESET && (rs >> i & 1)) v = all_<F>(1.f);
         const F e = mul_(bv, all_<F>(kLog2e));
         const F r = map_([](float t) { return ex2(-fabsf(t)); }, e), q = add_(r, all_<F>(1.f));
@@ -641,15 +649,14 @@ glr_bwd_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __rest
         sigmoid_pair(beta_of(i), si, ci);
         u[i] = mul_(rate, sg);
         a[i] = map_(ex2, mul_(u[i], all_<F>(kLog2e)));
-        const F a2 = mul_(a[i], a[i]);
         // 1 - a^2, kept off 0: a == 1 leaves its limits, m = 0 and (a^2 / m) u = 0, to 1e-18
         const F v = map_([](float t) { return fmaxf(t, 1e-36f); },
-                         one_minus_exp(mul_(u[i], all_<F>(-2.f)), a2));
+                         one_minus_square(mul_(u[i], all_<F>(-2.f)), a[i]));
         const F rv = map_(rsqrt_, v);
         F m = mul_(v, rv);
         if (RESET && (rs >> i & 1)) m = all_<F>(1.f);
         const F mi = mul_(m, si);
-        ring.q[w][i][lane] = mul_(a2, mul_(rv, rv));
+        ring.q[w][i][lane] = mul_(mul_(a[i], a[i]), mul_(rv, rv));
         ring.mi[w][i][lane] = mi;
         ring.put_gates(s, w, i, lane, ci);
         b = mul_(mi, x_of(i));
@@ -795,7 +802,7 @@ glr_step_kernel(const T* __restrict__ x, const G* __restrict__ g, const G* __res
       sigmoid2(in, i, unused);
       const float u = rate * s;
       a = ex2(u * kLog2e);
-      in = sqrt_(one_minus_exp(-2.f * u, a * a)) * i;
+      in = sqrt_(one_minus_square(-2.f * u, a)) * i;
     }
     const float s = fmaf(a, state[b * C + c], in * to_f<T>(x[b * st.xb + c]));
     state[b * C + c] = s;

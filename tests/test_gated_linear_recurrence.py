@@ -639,6 +639,30 @@ def test_rates_beyond_the_fp32_range():
             _within(o, want[:, t], 20 * U * want[:, t].abs(), "step")
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gates_near_1(dtype):
+    """a = e^{-y}, read as a single step's state from 1 without input, as the step's, and as the gradient
+    of the state in front: a long memory gathers its errors, so it has to be little more than rounded.
+    y = rate sigmoid(g) carries at most 20 U: 6 of softplus, 12 of the sigmoid with |g| <= 4, products.
+    The polynomial of 1 - a^2 adds 1.7 U of its value 2 y at most, half of which reaches a, what it is
+    subtracted from half a U of as much, and the exponential's own error (3 U) is left times y.
+    With the rounding of a itself: half a U + 26 y U."""
+    B, C = 64, 2048
+    v = _inputs(B, 1, C, dtype, dtype, True)
+    v["g"] = v["g"].clamp(-4, 4)
+    v["x"].zero_(), v["dh"].zero_(), v["h0"].fill_(1), v["dhT"].fill_(1)
+    v["decay"] = torch.log(torch.expm1(torch.logspace(-5, -0.7, C)))
+    y = torch.nn.functional.softplus(v["decay"].double()) * torch.sigmoid(v["g"][:, 0].double())
+    got = _run(v, 1.0)
+    state = v["h0"].to(DEV)
+    gated_linear_recurrence_step(*(v[k][:, 0].to(DEV) for k in ("x", "g", "beta")), state,
+                                 v["decay"].to(DEV))
+    for name, a in (("hT", got["hT"]), ("dh0", got["dh0"]), ("step", state)):
+        off = (a.double().cpu() - torch.exp(-y)).abs() / ((0.5 + 26 * y) * U)
+        assert float(off.max()) <= 1, (name, float(off.max()))
+
+
 # ---------------------------------------------------------------------------
 # refusals, on the CPU: nothing reaches the library
 # ---------------------------------------------------------------------------
