@@ -25,7 +25,7 @@
 //  - where slabs * B give every SM a CTA: from the neighbouring warp, as a chain through shared memory
 //    (an mbarrier a link), so that warps run ahead of one another and the gates of one overlap the
 //    walk of another (235 us against 266 us with a barrier for all warps when it came, forward at
-//    8 x 8192 x 2048 bf16 logits; 242 us now);
+//    8 x 8192 x 2048 bf16 logits; 240 us now);
 //  - with fewer slabs: up to 8 CTAs of a cluster take consecutive tiles, each warp's map is put
 //    together with those in front of it, and the CTAs exchange theirs as asynchronous stores that an
 //    mbarrier of the receiver counts (a cluster barrier waits for the outputs' stores too: backward
@@ -33,12 +33,12 @@
 // Inputs come through a ring of two rounds in shared memory (cp.async), which each warp fills and reads
 // by itself.  Every input is read once and every output written once.
 //
-// What bounds it (1 x B200, 8 x 8192 x 2048 bf16): gates as values 198 us forward and 355 us backward
+// What bounds it (1 x B200, 8 x 8192 x 2048 bf16): gates as values 200 us forward and 355 us backward
 // (floors 164 and 287 us at the measured rate of a copy), with fp32 gates 268 and 570 (246 and 451).
 // With logits an element takes five exponentials, reciprocals and roots, which alone take 150 us:
-// 242 us forward, 505 us backward (140 instructions for a pair of channels at 55 % of the issue rate, and
+// 240 us forward, 510 us backward (140 instructions for a pair of channels at 55 % of the issue rate, and
 // no more than 16 warps on an SM: two CTAs of 256 threads with up to 128 registers are all its
-// registers).  fp32 logits 316 and 730 us.  All of them lose an eighth to 256 CTAs on 148 SMs.
+// registers).  fp32 logits 315 and 735 us.  All of them lose an eighth to 256 CTAs on 148 SMs.
 
 #include <type_traits>
 
@@ -941,7 +941,7 @@ extern "C" int fo_glr_fwd(const void* x, const void* g, const void* beta, const 
     const bool wide = wide_ok(xs, 1, gs, 2, q, C, sizeof(T), sizeof(G));
     const int64_t ctas = B * slabs_of(C, two ? 2 : 1);
     // CTAs of a cluster until every SM has one: 242 us without, 292 with two at 8 x 8192 x 2048 bf16, where
-    // there are 256 CTAs as it is; 242 and 228 with 160 or 192 CTAs (batches of 5 and 6).
+    // there are 256 CTAs as it is; 242 and 228 with 160 or 192 CTAs (batches of 5 and 6).  (One comparison.)
     const int cl = cluster_for(ctas, (L + kFwdTile - 1) / kFwdTile, num_sms(), kMostCtas);
     return with_flags(two, decay, reset, [&](auto tw, auto lo, auto rs) {
       constexpr int V = tw && sizeof(G) == 2 ? 2 : 1;
